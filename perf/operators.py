@@ -1,0 +1,747 @@
+"""Performance cases of the paged 4-bit KV cache: the page plan of a ragged
+batch, the append (rotary positions on several axes, 4-bit rows) and the
+attention that reads the pages (sliding window, sink tokens), through the
+device-pointer entry points of include/draco_hip.h.
+
+A case is a dict of plain values.  `run` makes one pass: with `own` set
+through the library, otherwise in plain torch operations in 32 bits.
+
+The cache: a page holds `ps` tokens; per KV head K codes [ps][hd/2] bytes
+(dims 2j, 2j+1 in the low, high nibble of byte j), V codes
+[ps/16][hd/2][16 tokens] bytes (byte row b*16 + a: dims b*32 + a and
+b*32 + 16 + a), K scales [ps][hd/32] and V scales [ps/16][hd/32][16 tokens]
+in f16.  A code is E2M1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), a value is
+code * scale.
+"""
+import ctypes as ct
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+_PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dracomancer-llmengine_amd")
+device = "cuda"
+F16, F32 = 7, 9  # the library's type codes
+DTYPE = {"f32": torch.float32, "f16": torch.float16}
+CODE = {"f32": F32, "f16": F16}
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+# halfway between neighbouring codes, and whether a tie goes up (to the even code)
+MIDS = ((0.25, False), (0.75, True), (1.25, False), (1.75, True), (2.5, False), (3.5, True), (5.0, False))
+
+
+def listed():
+    return [
+        # a small server's decode step: 8 sessions, one token each
+        {"name": "plan_decode_8", "kind": "plan", "n_seq": 8, "ps": 16, "ctx": 1000, "chunk": 1, "pad": 0},
+        # a busy one's mixed step: 512 sessions, every eighth with a prompt chunk, rows padded for a captured graph
+        {"name": "plan_mixed_512", "kind": "plan", "n_seq": 512, "ps": 64, "ctx": 30000, "chunk": 1111, "pad": 777},
+        # sessions end and drafted tokens are taken back: pages of 300 sequences return to the free list
+        {"name": "release_300", "kind": "release", "n_seq": 300, "ps": 16, "ctx": 7000},
+        # one token of the small Q8_0 model: 15 q / 5 kv heads of 64, consecutive rotary pairs
+        {"name": "append_1_64", "kind": "append", "T": 1, "nh": 15, "nkv": 5, "hd": 64, "rot": 64, "axes": 1, "halves": False,
+         "ps": 16, "dtype": "f32", "chunked": False},
+        # a long prompt chunk of the MoE model's heads, 32 q / 4 kv of 128
+        {"name": "append_8192_128", "kind": "append", "T": 8192, "nh": 32, "nkv": 4, "hd": 128, "rot": 128, "axes": 1,
+         "halves": True, "ps": 64, "dtype": "f32", "chunked": True},
+        # an image's tokens in the hybrid model's heads (16 q / 2 kv of 256, 64 rotary dims), three axes, f16
+        {"name": "append_image_1037_256", "kind": "append", "T": 1037, "nh": 16, "nkv": 2, "hd": 256, "rot": 64, "axes": 3,
+         "halves": True, "ps": 32, "dtype": "f16", "chunked": True},
+        # decode of one short session, the flagship's heads (32 q / 8 kv of 64): the smallest call
+        {"name": "attn_decode_1x1000_64", "kind": "attn", "n_seq": 1, "q": 1, "len": 1000, "nh": 32, "nkv": 8, "hd": 64,
+         "ps": 16, "window": 0, "sink": 0, "dtype": "f32"},
+        # decode of a full batch at long, ragged contexts, the MoE model's heads
+        {"name": "attn_decode_64x16384_128", "kind": "attn", "n_seq": 64, "q": 1, "len": 16384, "nh": 32, "nkv": 4, "hd": 128,
+         "ps": 64, "window": 0, "sink": 0, "dtype": "f32"},
+        # drafted tokens checked in one pass at long context with a sliding window and sinks, hybrid model's heads
+        {"name": "attn_draft_24x20011_256", "kind": "attn", "n_seq": 24, "q": 5, "len": 20011, "nh": 16, "nkv": 2, "hd": 256,
+         "ps": 32, "window": 6001, "sink": 4, "dtype": "f16"},
+        # a prompt chunk over a cached prefix, f16 rows
+        {"name": "attn_chunk_2048_128", "kind": "attn", "n_seq": 1, "q": 2048, "len": 8192, "nh": 32, "nkv": 4, "hd": 128,
+         "ps": 64, "window": 0, "sink": 0, "dtype": "f16"},
+        # a ragged batch of prompts, odd lengths, fp32 rows, the flagship's heads, a window
+        {"name": "attn_prompts_5x777_64", "kind": "attn", "n_seq": 5, "q": 777, "len": 777, "nh": 32, "nkv": 8, "hd": 64,
+         "ps": 16, "window": 500, "sink": 2, "dtype": "f32"},
+        # one layer's whole decode step: plan, append, attention over 40 sessions
+        {"name": "step_40x3000_128", "kind": "step", "n_seq": 40, "len": 3000, "nh": 32, "nkv": 8, "hd": 128, "ps": 32,
+         "window": 0, "sink": 0, "dtype": "f32"},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["plan", "release", "append", "append", "attn", "attn", "attn", "attn", "step"])
+    ps = rng.choice([16, 32, 64, 128])
+    hd = rng.choice([64, 128, 256])
+    nkv = rng.choice([1, 2, 4, 5, 8])
+    nh = nkv * rng.choice([1, 3, 4, 8] if hd < 256 else [1, 2, 4, 8])
+    dtype = rng.choice(["f32", "f16"])
+    if kind == "plan":
+        return {"kind": kind, "n_seq": _log(rng, 1, 512), "ps": ps, "ctx": _log(rng, 100, 30000),
+                "chunk": rng.choice([1, _log(rng, 2, 1100)]), "pad": rng.choice([0, rng.randint(1, 999)])}
+    if kind == "release":
+        return {"kind": kind, "n_seq": _log(rng, 1, 500), "ps": ps, "ctx": _log(rng, 100, 12000)}
+    if kind == "append":
+        chunked = rng.random() < 0.6
+        return {"kind": kind, "T": _log(rng, 1, 8000 if chunked else 300), "nh": nh, "nkv": nkv, "hd": hd,
+                "rot": rng.choice([0, hd // 4, hd]), "axes": rng.choice([1, 2, 3]), "halves": rng.random() < 0.5, "ps": ps,
+                "dtype": dtype, "chunked": chunked}
+    window, sink = rng.choice([(0, 0), (_log(rng, 16, 8000), rng.choice([0, 1, 4, 40]))])
+    if kind == "step":
+        return {"kind": kind, "n_seq": _log(rng, 1, 60), "len": _log(rng, 10, 6000), "nh": nh, "nkv": nkv, "hd": hd, "ps": ps,
+                "window": window, "sink": sink, "dtype": dtype}
+    how = rng.choice(["decode", "decode", "draft", "chunk"])
+    if how == "decode":
+        n_seq = _log(rng, 1, 64)
+        return {"kind": kind, "n_seq": n_seq, "q": 1, "len": _log(rng, 1, min(120000, 500000000 // (n_seq * nkv * hd))),
+                "nh": nh, "nkv": nkv, "hd": hd, "ps": ps, "window": window, "sink": sink, "dtype": dtype}
+    if how == "draft":
+        q, n_seq = rng.randint(2, 16), _log(rng, 1, 32)
+        return {"kind": kind, "n_seq": n_seq, "q": q, "len": _log(rng, 20, min(30000, 200000000 // (n_seq * nkv * hd))),
+                "nh": nh, "nkv": nkv, "hd": hd, "ps": ps, "window": window, "sink": sink, "dtype": dtype}
+    q, n_seq = _log(rng, 17, 2000), rng.randint(1, 4)
+    more = 60000000000 // (n_seq * q * nh * hd) - q
+    return {"kind": kind, "n_seq": n_seq, "q": q, "len": q + rng.choice([0, _log(rng, 1, max(1, min(5000, more)))]), "nh": nh,
+            "nkv": nkv, "hd": hd, "ps": ps, "window": window, "sink": sink, "dtype": dtype}
+
+
+# ---- what a case means: lengths by a fixed rule, so that its work is known -----
+
+def _lens(case):
+    """The batch's (cached tokens before the step, new tokens), per sequence."""
+    n = case["n_seq"]
+    part = [((s * 0.6180339887) % 1.0) for s in range(n)]  # ragged: evenly spread in (0, 1)
+    if case["kind"] in ("plan", "release"):
+        old = [int(case["ctx"] * f) for f in part[1:] + [0.999]]
+        if case["kind"] == "release":
+            return old, [0] * n
+        if case["chunk"] == 1:
+            return old, [1] * n
+        # every eighth sequence brings a chunk, every fifth of the others nothing, the rest one token
+        return old, [1 + int((case["chunk"] - 1) * f) if s % 8 == 0 else int(s % 5 != 0) for s, f in enumerate(part)]
+    if case["kind"] == "step":
+        tot = [max(1, int(case["len"] * (1.0 - 0.7 * f))) for f in part]
+        return [t - 1 for t in tot], [1] * n
+    tot = [max(1, int(case["len"] * (1.0 - 0.7 * f))) for f in part]
+    new = [min(t, max(1, int(case["q"] * (1.0 - (0.7 if case["q"] > 16 else 0.0) * f)))) for t, f in zip(tot, part)]
+    return [t - q for t, q in zip(tot, new)], new
+
+
+def _visible(pos, length, window, sink):
+    """Keys that the query at `pos` sees."""
+    hi = min(pos, length - 1)
+    lo = max(0, pos - window + 1) if window > 0 else 0
+    return max(0, hi - lo + 1) + min(sink, lo, hi + 1)
+
+
+def work(case):
+    k = case["kind"]
+    if k in ("plan", "release"):
+        old, new = _lens(case)
+        ps, tok = case["ps"], sum(new) + case.get("pad", 0)
+        if k == "plan":
+            pages = sum(-(-(a + b) // ps) - -(-a // ps) for a, b in zip(old, new))
+            return {"bytes": 16 * len(old) + 8 * tok + 8 * pages, "flops": 0}
+        pages = sum(-(-a // ps) - -(-b // ps) for a, b in zip(old, _keep(old)))
+        return {"bytes": 12 * len(old) + 12 * pages, "flops": 0}
+    if k == "append":
+        e, T, w = (4 if case["dtype"] == "f32" else 2), case["T"], case["hd"]
+        return {"bytes": T * (2 * case["nh"] * w * e + 2 * case["nkv"] * (w * e + w * 9 // 16) + 4 * case["axes"] + 4),
+                "flops": 3 * T * (case["nh"] + case["nkv"]) * case["rot"]}
+    old, new = _lens(case)
+    e, hd = (4 if case["dtype"] == "f32" else 2), case["hd"]
+    seen = keys = 0
+    for a, q in zip(old, new):
+        lo = max(0, a - case["window"] + 1) if case["window"] > 0 else 0
+        keys += a + q - lo + min(case["sink"], lo)
+        seen += sum(_visible(p, a + q, case["window"], case["sink"]) for p in range(a, a + q))
+    T = sum(new)
+    b = keys * case["nkv"] * hd * 9 // 8 + 2 * T * case["nh"] * hd * e
+    if k == "step":
+        b += T * (2 * case["nh"] * hd * e + 2 * case["nkv"] * (hd * e + hd * 9 // 16)) + 24 * case["n_seq"]
+    return {"bytes": b, "flops": 4 * hd * seen * case["nh"]}
+
+
+def _keep(old):
+    """What a release leaves: every third sequence ends, the others lose a few drafted tokens."""
+    return [0 if s % 3 == 0 else max(0, a - 40 - s % 7) for s, a in enumerate(old)]
+
+
+# ---- inputs ------------------------------------------------------------------
+
+class _State:
+    def __init__(self, **kw):
+        self.__dict__.update(kw)
+        self.call = None  # the library call's descriptors, made on the first pass
+
+
+def _gen(seed):
+    return torch.Generator(device=device).manual_seed(int(seed) % (1 << 62))
+
+
+def _ints(v):
+    return torch.tensor(list(v), dtype=torch.int32, device=device)
+
+
+def _head_bytes(hd, ps):
+    return ps * (hd + hd // 8)
+
+
+def _round9(t):
+    """A scale: t (64 bits) to 9 significant bits and a multiple of 2^-23, ties to even, at most 10912."""
+    up = torch.clamp(torch.frexp(t)[1].long() - 9, min=-23)
+    ulp = ((up + 1023) << 52).view(torch.float64)  # 2^up
+    return torch.clamp(torch.round(t / ulp) * ulp, max=10912.0)
+
+
+def _cache(gen, n_pages, nkv, hd, ps):
+    """Pages as decoding fills them: codes of normal rows (about uniform), scales of rows whose blocks differ in size."""
+    pages = torch.randint(0, 256, (n_pages, nkv, _head_bytes(hd, ps)), generator=gen, dtype=torch.uint8, device=device)
+    n = ps * hd // 32
+    s = torch.exp(0.4 * torch.randn(n_pages, nkv, 2 * n, generator=gen, device=device)) * 0.35
+    pages[:, :, ps * hd:] = _round9(s.double()).half().view(torch.uint8)
+    return pages
+
+
+def _tables(gen, case, old, new, spare):
+    """Block tables over a shuffled pool, the free list and the pool's size: pages of the cached tokens are in place."""
+    ps = case["ps"]
+    have = [-(-a // ps) for a in old]
+    need = [-(-(a + q) // ps) for a, q in zip(old, new)]
+    n_pages = sum(need) + spare
+    width = max(max(need), 1) + 2
+    order = torch.randperm(n_pages, generator=gen, device=device).to(torch.int32)
+    at = torch.full((len(old), width), -1, dtype=torch.int64)
+    k = 0
+    for s, h in enumerate(have):
+        at[s, :h] = torch.arange(k, k + h)
+        k += h
+    at = at.to(device)
+    table = torch.where(at >= 0, order[at.clamp(min=0)], torch.full_like(order[:1], -1))
+    n_free = n_pages - k
+    free = torch.full((n_pages,), -1, dtype=torch.int32, device=device)
+    free[:n_free] = order[k:]
+    return table, free, _ints([n_free]), n_pages
+
+
+def _rope_table(rows, rot, base=500000.0):
+    """cos, sin [rows][rot/2][2] fp32, angles in 64 bits."""
+    inv = base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
+    ang = torch.arange(rows, dtype=torch.float64, device=device)[:, None] * inv[None, :]
+    return torch.stack([torch.cos(ang), torch.sin(ang)], -1).float().contiguous()
+
+
+def _prepare_pages(case, seed):
+    gen = _gen(seed)
+    old, new = _lens(case)
+    n = len(old)
+    s = _State(case=case, n=n)
+    s.table, s.free, s.n_free, s.n_pages = _tables(gen, case, old, new, 64)
+    s.kv_len, s.q_len = _ints(old), _ints(new)
+    s.kv_out, s.n_free_out = torch.zeros_like(s.kv_len), torch.zeros_like(s.n_free)
+    s.status = torch.zeros(2, dtype=torch.int32, device=device)
+    s.work = torch.zeros(4, dtype=torch.int32, device=device)
+    if case["kind"] == "release":
+        s.keep = _ints(_keep(old))
+        # the pool as it was taken: the table's pages are not in the list
+        s.table_out, s.free_out = s.table.clone(), s.free.clone()
+        return s
+    s.n_tok = sum(new) + case.get("pad", 0)
+    s.cu = torch.zeros(n + 1, dtype=torch.int32, device=device)
+    s.pos, s.slot = (torch.zeros(s.n_tok, dtype=torch.int32, device=device) for _ in range(2))
+    return s
+
+
+def _prepare_append(case, seed):
+    gen = _gen(seed)
+    T, hd, ps, dt = case["T"], case["hd"], case["ps"], DTYPE[case["dtype"]]
+    n_pages = (T if not case["chunked"] else -(-T // ps)) + 3
+    s = _State(case=case, n_pages=n_pages)
+    s.pages = torch.zeros(n_pages, case["nkv"], _head_bytes(hd, ps), dtype=torch.uint8, device=device)
+    order = torch.randperm(n_pages, generator=gen, device=device)
+    t = torch.arange(T, device=device)
+    if case["chunked"]:  # one prompt's tokens, from the middle of a page on
+        first = ps // 3 if T + ps // 3 <= (n_pages - 1) * ps else 0
+        slot = order[(t + first) // ps] * ps + (t + first) % ps
+    else:  # one token each of T sessions
+        slot = order[t] * ps + torch.randint(0, ps, (T,), generator=gen, device=device)
+    s.slot = slot.to(torch.int32)
+    s.q, s.k, s.v = (torch.randn(T, h, hd, generator=gen, device=device) for h in (case["nh"], case["nkv"], case["nkv"]))
+    s.k *= torch.exp(0.8 * torch.randn(case["nkv"], hd, generator=gen, device=device))  # channels of differing size
+    s.q, s.k, s.v = s.q.to(dt), s.k.to(dt), s.v.to(dt)
+    rows = 20000
+    # text: one running position; images: time, height and width of a patch
+    base = torch.randint(0, rows - 9000, (1,), generator=gen, device=device)
+    s.pos = torch.stack([base + t, base + (t // 64) % 512, base + t % 64][:case["axes"]]).to(torch.int32).contiguous()
+    s.rows = rows
+    s.table = _rope_table(rows, case["rot"]) if case["rot"] else None
+    s.axis = [i % case["axes"] for i in range(case["rot"] // 2)]  # axes interleaved over the pairs
+    s.q_out = torch.zeros_like(s.q)
+    s.k_val, s.v_val = (torch.zeros(T, case["nkv"], hd, device=device) for _ in range(2))
+    return s
+
+
+def _prepare_attn(case, seed):
+    gen = _gen(seed)
+    old, new = _lens(case)
+    n, hd, dt = len(old), case["hd"], DTYPE[case["dtype"]]
+    whole = [a + q for a, q in zip(old, new)]
+    s = _State(case=case, n=n, n_tok=sum(new), max_q=max(new), max_len=max(whole))
+    # attention alone: the chunk's rows are in the pages already
+    s.table, s.free, s.n_free, s.n_pages = _tables(gen, case, whole, [0] * n, 5)
+    s.pages = _cache(gen, s.n_pages, case["nkv"], hd, case["ps"])
+    s.kv_len, s.q_len = _ints(whole), _ints(new)
+    s.cu = _ints([sum(new[:i]) for i in range(n + 1)]) if n < 2000 else None
+    s.q = (1.5 * torch.randn(s.n_tok, case["nh"], hd, generator=gen, device=device)).to(dt)
+    s.out = torch.zeros_like(s.q)
+    return s
+
+
+def _prepare_step(case, seed):
+    gen = _gen(seed)
+    s = _prepare_pages(case, seed)
+    n, hd, dt = s.n, case["hd"], DTYPE[case["dtype"]]
+    s.n_tok, s.max_q, s.max_len, s.rows = n, 1, case["len"], case["len"] + 8
+    s.pages = _cache(gen, s.n_pages, case["nkv"], hd, case["ps"])
+    s.q, s.k, s.v = ((1.5 * torch.randn(n, h, hd, generator=gen, device=device)).to(dt)
+                     for h in (case["nh"], case["nkv"], case["nkv"]))
+    s.rope = _rope_table(s.rows, hd)
+    s.q_out, s.out = torch.zeros_like(s.q), torch.zeros_like(s.q)
+    return s
+
+
+def prepare(case, seed):
+    return {"plan": _prepare_pages, "release": _prepare_pages, "append": _prepare_append, "attn": _prepare_attn,
+            "step": _prepare_step}[case["kind"]](case, seed)
+
+
+# ---- the library's calls --------------------------------------------------------
+
+_streams = []
+
+
+def _lib():
+    if _PKG not in sys.path:
+        sys.path.insert(0, _PKG)
+    from dracohip import lib
+    return lib
+
+
+def _stream():
+    """The serving loop's stream."""
+    if not _streams:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        _streams.append(s)
+    return _streams[0].cuda_stream
+
+
+def _own_plan(s):
+    L = _lib()
+    c = s.case
+    a = L.KvPlan(n_seq=s.n, max_blocks=s.table.shape[1], n_pages=s.n_pages, page_size=c["ps"], n_tok=s.n_tok,
+                 block_table=s.table.data_ptr(), kv_len=s.kv_len.data_ptr(), q_len=s.q_len.data_ptr(),
+                 free_list=s.free.data_ptr(), n_free=s.n_free.data_ptr(), cu_q=s.cu.data_ptr(), pos=s.pos.data_ptr(),
+                 slot=s.slot.data_ptr(), kv_len_out=s.kv_out.data_ptr(), n_free_out=s.n_free_out.data_ptr(),
+                 status=s.status.data_ptr(), work=s.work.data_ptr())
+    return L.load().draco_kv_plan, ct.byref(a)
+
+
+def _own_release(s):
+    L = _lib()
+    a = L.KvRelease(n_seq=s.n, max_blocks=s.table.shape[1], n_pages=s.n_pages, page_size=s.case["ps"],
+                    block_table=s.table.data_ptr(), block_table_out=s.table_out.data_ptr(), kv_len=s.kv_len.data_ptr(),
+                    keep=s.keep.data_ptr(), free_list=s.free_out.data_ptr(), n_free=s.n_free.data_ptr(),
+                    kv_len_out=s.kv_out.data_ptr(), n_free_out=s.n_free_out.data_ptr(), work=s.work.data_ptr())
+    return L.load().draco_kv_release, ct.byref(a)
+
+
+def _own_cache(s):
+    c = s.case
+    return _lib().Kv4(data=s.pages.data_ptr(), n_pages=s.n_pages, page_size=c["ps"], n_kv=c["nkv"], head_dim=c["hd"])
+
+
+def _own_append(s, T, table, rows, axis, n_axes, halves):
+    L, c = _lib(), s.case
+    w = c["hd"]
+    a = L.Kv4Append(code=CODE[c["dtype"]], n_tok=T, n_head=c["nh"], q=s.q.data_ptr(), q_out=s.q_out.data_ptr(),
+                    k=s.k.data_ptr(), v=s.v.data_ptr(), q_stride=c["nh"] * w, q_out_stride=c["nh"] * w,
+                    k_stride=c["nkv"] * w, v_stride=c["nkv"] * w, slot=s.slot.data_ptr(),
+                    rot=2 * len(axis), pairing=int(halves), n_axes=n_axes, pos=s.pos.data_ptr(), pos_stride=T,
+                    table=table.data_ptr() if table is not None else None, table_rows=rows)
+    for i, x in enumerate(axis):
+        a.axis[i] = x
+    return L.load().draco_kv4_append, ct.byref(_own_cache(s)), ct.byref(a)
+
+
+def _own_attn(s, q, kv_len):
+    L, c = _lib(), s.case
+    w = c["hd"]
+    a = L.Kv4Attn(code=CODE[c["dtype"]], n_seq=s.n, n_tok=s.n_tok, max_q=s.max_q, max_len=s.max_len, n_head=c["nh"],
+                  window=c["window"], sink=c["sink"], scale=w ** -0.5, max_blocks=s.table.shape[1], q=q.data_ptr(),
+                  out=s.out.data_ptr(), q_stride=c["nh"] * w, out_stride=c["nh"] * w, cu_q=s.cu.data_ptr(),
+                  kv_len=kv_len.data_ptr(), block_table=s.table.data_ptr())
+    cache = _own_cache(s)
+    need = L.load().draco_kv4_attn_workspace(ct.byref(cache), ct.byref(a))
+    s.attn_work = torch.zeros(max(16, need), dtype=torch.uint8, device=device)
+    torch.cuda.current_stream().synchronize()  # the workspace is cleared before another stream uses it
+    a.work, a.work_bytes = s.attn_work.data_ptr(), need
+    return L.load().draco_kv4_attn, ct.byref(cache), ct.byref(a)
+
+
+def _call(fn, *args):
+    rc = fn(*args, _stream())
+    if rc:
+        _lib().check(rc, fn.__name__)
+
+
+def _run_own(s):
+    k = s.case["kind"]
+    if k == "plan":
+        s.call = s.call or [_own_plan(s)]
+    elif k == "release":
+        s.call = s.call or [_own_release(s)]
+    elif k == "append":
+        c = s.case
+        if s.call is None:
+            lib = _lib().load()
+            s.call = [_own_append(s, c["T"], s.table, s.rows, s.axis, c["axes"], c["halves"]),
+                      (lib.draco_kv4_read, ct.byref(_own_cache(s)), s.slot.data_ptr(), c["T"], s.k_val.data_ptr(),
+                       s.v_val.data_ptr())]
+    elif k == "attn":
+        s.call = s.call or [_own_attn(s, s.q, s.kv_len)]
+    else:
+        s.call = s.call or [_own_plan(s), _own_append(s, s.n, s.rope, s.rows, [0] * (s.case["hd"] // 2), 1, True),
+                            _own_attn(s, s.q_out, s.kv_out)]
+    for c in s.call:
+        _call(*c)
+
+
+# ---- the plain forms ------------------------------------------------------------
+
+def _plain_plan(s):
+    ps, n = s.case["ps"], s.n
+    old, new, free = s.kv_len.long(), s.q_len.long(), s.n_free.long()
+    cu = torch.cat([torch.zeros_like(free), torch.cumsum(new, 0)])
+    have, want = (old + ps - 1) // ps, (old + new + ps - 1) // ps
+    last = torch.cumsum(want - have, 0)
+    fits = (old + new <= s.table.shape[1] * ps) & (cu[1:] <= s.n_tok)
+    ok = fits & ((want == have) | (last <= free))
+    # the new pages: block b of sequence i is the (last - want + b)-th page taken
+    b = torch.arange(s.table.shape[1], device=old.device)[None, :]
+    take = (b >= have[:, None]) & (b < want[:, None]) & ok[:, None]
+    page = s.free[(free - 1 - ((last - want)[:, None] + b)).clamp(0, s.n_pages - 1)]
+    s.table.copy_(torch.where(take, page, s.table))
+    t = torch.arange(s.n_tok, device=old.device)
+    i = torch.searchsorted(cu[1:], t, right=True)
+    real = i < n
+    i = i.clamp(max=n - 1)
+    real = real & ok[i]
+    pos = old[i] + t - cu[i]
+    page = s.table[i, (pos // ps).clamp(0, s.table.shape[1] - 1)].long()
+    none = torch.full_like(pos, -1)
+    s.slot.copy_(torch.where(real, page * ps + pos % ps, none))
+    s.pos.copy_(torch.where(real, pos, none))
+    s.cu.copy_(cu.clamp(max=s.n_tok))
+    s.kv_out.copy_(old + torch.where(ok, new, torch.zeros_like(new)))
+    s.n_free_out.copy_(free - torch.where(ok, want - have, torch.zeros_like(have)).sum())
+    s.status[0] = (~ok).sum()
+
+
+def _plain_release(s):
+    ps = s.case["ps"]
+    old, n_free = s.kv_len.long(), s.n_free.long()
+    keep = torch.minimum(s.keep.long().clamp(min=0), old)
+    have, want = (old + ps - 1) // ps, (keep + ps - 1) // ps
+    last = torch.cumsum(have - want, 0)
+    b = torch.arange(s.table.shape[1], device=old.device)[None, :]
+    go = (b >= want[:, None]) & (b < have[:, None])
+    # back in the reverse order of the taking
+    at = n_free + last[-1] - 1 - ((last - have)[:, None] + b)
+    spill = torch.full_like(at, s.n_pages)
+    room = torch.cat([s.free_out, s.free_out[:1]])
+    room[torch.where(go, at, spill)] = s.table
+    s.free_out.copy_(room[:-1])
+    s.table_out.copy_(torch.where(go, torch.full_like(s.table, -1), s.table))
+    s.kv_out.copy_(keep)
+    s.n_free_out.copy_(n_free + last[-1])
+
+
+def _plain_rope(x, table, pos, axis, halves):
+    """x [T][heads][hd], the leading 2 * len(axis) dims rotated pair by pair (products in 64 bits)."""
+    rot = 2 * len(axis)
+    if not rot:
+        return x.double()
+    at = pos[axis].long()                                      # [pairs][T]
+    cs = table[at, torch.arange(rot // 2, device=x.device)[:, None]].double().transpose(0, 1)
+    c, n = cs[:, None, :, 0], cs[:, None, :, 1]
+    y = x.double()
+    a, b = (y[..., :rot // 2], y[..., rot // 2:rot]) if halves else (y[..., 0:rot:2], y[..., 1:rot:2])
+    u, w = a * c - b * n, a * n + b * c
+    turned = torch.cat([u, w], -1) if halves else torch.stack([u, w], -1).flatten(-2)
+    return torch.cat([turned, y[..., rot:]], -1)
+
+
+def _plain_quant(x):
+    """Rows in 4 bits: (codes, scales) of blocks of 32; the codes by exact comparisons with the scaled midpoints."""
+    b = x.float().unflatten(-1, (-1, 32))
+    a = b.abs()
+    top = a.amax(-1, keepdim=True).double()
+    s = _round9(top / torch.full_like(top, 6.0)).float()  # (a scalar divisor becomes a product with its reciprocal)
+    code = sum((a >= m * s if up else a > m * s).to(torch.uint8) for m, up in MIDS)
+    code = torch.where(s > 0, code, torch.zeros_like(code)) | ((b < 0).to(torch.uint8) << 3)
+    return code.flatten(-2), s.squeeze(-1)
+
+
+def _values(code, scale):
+    lut = torch.tensor(E2M1 + tuple(-x for x in E2M1), device=code.device)
+    return (lut[code.int()].unflatten(-1, (-1, 32)) * scale.float()[..., None]).flatten(-2)
+
+
+def _plain_write(s, k, v):
+    """Rows into the pages, in the library's layout; the values they stand for."""
+    c, hd, ps = s.case, s.case["hd"], s.case["ps"]
+    (kc, ks), (vc, vs) = _plain_quant(k), _plain_quant(v)
+    page, off = (s.slot // ps).long(), (s.slot % ps).long()
+    kcodes = s.pages[:, :, :ps * hd // 2].unflatten(2, (ps, hd // 2))
+    vcodes = s.pages[:, :, ps * hd // 2:ps * hd].unflatten(2, (ps // 16, hd // 2, 16))
+    m = ps * hd // 16
+    ksc = s.pages[:, :, ps * hd:ps * hd + m].unflatten(2, (ps, hd // 32, 2))
+    vsc = s.pages[:, :, ps * hd + m:].unflatten(2, (ps // 16, hd // 32, 16, 2))
+    kcodes[page, :, off] = kc[..., 0::2] | (kc[..., 1::2] << 4)
+    vb = vc.unflatten(-1, (hd // 32, 2, 16))
+    vcodes[page, :, off // 16, :, off % 16] = (vb[..., 0, :] | (vb[..., 1, :] << 4)).flatten(-2)
+    ksc[page, :, off] = ks.half().contiguous().view(torch.uint8).unflatten(-1, (-1, 2))
+    vsc[page, :, off // 16, :, off % 16] = vs.half().contiguous().view(torch.uint8).unflatten(-1, (-1, 2))
+    return _values(kc, ks), _values(vc, vs)
+
+
+def _plain_append(s, table, axis, halves):
+    s.q_out.copy_(_plain_rope(s.q, table, s.pos, axis, halves))
+    return _plain_write(s, _plain_rope(s.k, table, s.pos, axis, halves), s.v)
+
+
+def _plain_rows(s, blocks):
+    """The cached K and V values [n_seq][kv heads][tokens][hd] of each sequence's first `blocks` pages."""
+    hd, ps = s.case["hd"], s.case["ps"]
+    p = s.pages[s.table[:, :blocks].clamp(min=0).long()].transpose(1, 2)   # [n_seq][nkv][blocks][bytes]
+    m = ps * hd // 16
+    half = lambda x: x.contiguous().view(torch.float16)  # noqa: E731
+    kb = p[..., :ps * hd // 2].unflatten(-1, (ps, hd // 2))
+    kc = torch.stack([kb & 15, kb >> 4], -1).flatten(-2)
+    ks = half(p[..., ps * hd:ps * hd + m]).unflatten(-1, (ps, hd // 32))
+    vb = p[..., ps * hd // 2:ps * hd].unflatten(-1, (ps // 16, hd // 32, 16, 16)).movedim(-1, -3)
+    vc = torch.stack([vb & 15, vb >> 4], -2).flatten(-3).flatten(-3, -2)
+    vs = half(p[..., ps * hd + m:]).unflatten(-1, (ps // 16, hd // 32, 16)).transpose(-1, -2).flatten(-3, -2)
+    return _values(kc, ks).flatten(2, 3), _values(vc, vs).flatten(2, 3)
+
+
+def _plain_attn(s, q, kv_len):
+    c = s.case
+    Q, n, nkv, hd, g = s.max_q, s.n, c["nkv"], c["hd"], c["nh"] // c["nkv"]
+    blocks = -(-s.max_len // c["ps"])
+    k, v = _plain_rows(s, blocks)
+    i = torch.arange(Q, device=q.device)[None, :]
+    real = i < s.q_len.long()[:, None]                                      # [n][Q]
+    row = (s.cu[:-1].long()[:, None] + i).clamp(max=s.n_tok - 1)
+    x = q[row].float().unflatten(2, (nkv, g)).permute(0, 2, 1, 3, 4).reshape(n, nkv, Q * g, hd)
+    sc = torch.matmul(x * hd ** -0.5, k.transpose(2, 3).contiguous())
+    pos = (kv_len.long() - s.q_len.long())[:, None] + i                     # [n][Q]
+    j = torch.arange(k.shape[2], device=q.device)[None, None, :]
+    see = (j <= pos[..., None]) & (j < kv_len.long()[:, None, None])
+    if c["window"] > 0:
+        see &= (j > pos[..., None] - c["window"]) | (j < c["sink"])
+    sc = sc.unflatten(2, (Q, g)).masked_fill_(~see[:, None, :, None, :], -math.inf)
+    top = sc.amax(-1, keepdim=True)
+    sc = torch.exp(sc.sub_(torch.where(torch.isfinite(top), top, torch.zeros_like(top))))
+    den = sc.sum(-1, keepdim=True)
+    o = torch.matmul(sc.flatten(2, 3), v).unflatten(2, (Q, g)) / torch.where(den > 0, den, torch.ones_like(den))
+    o = o.permute(0, 2, 1, 3, 4).flatten(2, 3).to(q.dtype)                  # [n][Q][nh][hd]
+    s.out[row[real]] = o[real]
+
+
+def _run_plain(s):
+    k, c = s.case["kind"], s.case
+    if k == "plan":
+        _plain_plan(s)
+    elif k == "release":
+        _plain_release(s)
+    elif k == "append":
+        kv, vv = _plain_append(s, s.table, s.axis, c["halves"])
+        s.k_val.copy_(kv)
+        s.v_val.copy_(vv)
+    elif k == "attn":
+        _plain_attn(s, s.q, s.kv_len)
+    else:
+        _plain_plan(s)
+        pos, s.pos = s.pos, s.pos[None]
+        _plain_append(s, s.rope, [0] * (c["hd"] // 2), True)
+        s.pos = pos
+        _plain_attn(s, s.q_out, s.kv_out)
+
+
+def run(state):
+    s, k = state, state.case["kind"]
+    if own:
+        _run_own(s)
+    else:
+        _run_plain(s)
+    if k == "plan":
+        return {"cu_q": s.cu, "pos": s.pos, "slot": s.slot, "block_table": s.table, "kv_len": s.kv_out, "n_free": s.n_free_out,
+                "status": s.status}
+    if k == "release":
+        return {"block_table": s.table_out, "free_list": s.free_out, "kv_len": s.kv_out, "n_free": s.n_free_out}
+    if k == "append":
+        return {"q": s.q_out, "k": s.k_val, "v": s.v_val}
+    if k == "attn":
+        return {"out": s.out}
+    return {"q": s.q_out, "out": s.out, "slot": s.slot, "kv_len": s.kv_out}
+
+
+# ---- the definitions, in 64 bits --------------------------------------------------
+
+def _exact_plan(s):
+    c, ps, n, width = s.case, s.case["ps"], s.n, s.table.shape[1]
+    old, new, free, table = s.kv_len.tolist(), s.q_len.tolist(), s.free.tolist(), s.table.tolist()
+    left = start = s.n_free.tolist()[0]
+    cu, pos, slot, after, refused, taken = [0], [], [], [], 0, 0
+    for i in range(n):
+        a, q = old[i], new[i]
+        need = -(-(a + q) // ps) - -(-a // ps)
+        taken += need
+        ok = a + q <= width * ps and cu[-1] + q <= s.n_tok and (need == 0 or taken <= start)
+        refused += not ok
+        cu.append(cu[-1] + q)
+        for b in range(-(-a // ps), -(-(a + q) // ps) if ok else 0):
+            left -= 1
+            table[i][b] = free[left]
+        for p in range(a, a + q):
+            pos.append(p if ok else -1)
+            slot.append(table[i][p // ps] * ps + p % ps if ok else -1)
+        after.append(a + q if ok else a)
+    fill = [-1] * (s.n_tok - len(pos))
+    return {"cu_q": _ints(cu), "pos": _ints(pos + fill), "slot": _ints(slot + fill), "block_table": _ints(sum(table, [])).reshape(n, width),
+            "kv_len": _ints(after), "n_free": _ints([left]), "status": _ints([refused, 0])}
+
+
+def _exact_release(s):
+    ps, table, free = s.case["ps"], s.table.tolist(), s.free.tolist()
+    back, kept = [], []
+    for i, (a, k) in enumerate(zip(s.kv_len.tolist(), s.keep.tolist())):
+        k = min(a, k)
+        kept.append(k)
+        for b in range(-(-k // ps), -(-a // ps)):
+            back.append(table[i][b])
+            table[i][b] = -1
+    n = s.n_free.tolist()[0]
+    free[n:n + len(back)] = back[::-1]
+    return {"block_table": _ints(sum(table, [])).reshape(s.n, -1), "free_list": _ints(free), "kv_len": _ints(kept),
+            "n_free": _ints([n + len(back)])}
+
+
+def _exact_turn(x, s, table, axis, halves):
+    x = x.double().clone()
+    half = len(axis)
+    for i, ax in enumerate(axis):
+        p = s.pos.reshape(-1, x.shape[0])[ax].long()
+        co, si = table[p, i, 0].double()[:, None], table[p, i, 1].double()[:, None]
+        d0, d1 = (i, i + half) if halves else (2 * i, 2 * i + 1)
+        a, b = x[:, :, d0].clone(), x[:, :, d1].clone()
+        x[:, :, d0], x[:, :, d1] = a * co - b * si, b * co + a * si
+    return x
+
+
+def _exact_held(x):
+    """The values that 4 bits hold for rows x: the nearest of the scaled codes, ties to the even code."""
+    b = x.float().double().unflatten(-1, (-1, 32))
+    want = b.abs().amax(-1, keepdim=True)
+    want = want / torch.full_like(want, 6.0)
+    two = torch.tensor([2.0 ** e for e in range(-15, 128)], dtype=torch.float64, device=x.device)
+    step = two[(torch.searchsorted(two, want, right=True) - 1).clamp(min=0)] / 256.0
+    s = torch.round(want / step) * step
+    grid = torch.tensor(E2M1, dtype=torch.float64, device=x.device)
+    # even codes first: the first of two equally near ones is the even one
+    grid = torch.cat([grid[0::2], grid[1::2]])
+    near, best = torch.full_like(b, math.inf), torch.zeros_like(b)
+    for g in grid:
+        d = (b.abs() - g * s).abs()
+        best = torch.where(d < near, g * s, best)
+        near = torch.minimum(near, d)
+    return (torch.sign(b) * best).flatten(-2)
+
+
+def _exact_rows(s, i, length, extra=None):
+    """Sequence i's first `length` K and V rows [nkv][length][hd] in 64 bits, read value by value from the page layout."""
+    c, hd, ps = s.case, s.case["hd"], s.case["ps"]
+    j, d = torch.arange(length, device=device)[:, None], torch.arange(hd, device=device)[None, :]
+    page, off = s.table[i].long()[j // ps], j % ps
+    flat = s.pages.flatten(1)
+    lut = torch.tensor(E2M1 + tuple(-x for x in E2M1), dtype=torch.float64, device=device)
+    got = []
+    for v in (0, 1):
+        rows = []
+        for h in range(c["nkv"]):
+            base = h * _head_bytes(hd, ps)
+            if v:
+                byte = base + ps * hd // 2 + (off // 16) * 8 * hd + ((d // 32) * 16 + d % 16) * 16 + off % 16
+                up = (d // 16) % 2
+                sc = base + ps * hd + ps * hd // 16 + ((off // 16) * (hd // 32) * 16 + (d // 32) * 16 + off % 16) * 2
+            else:
+                byte = base + off * (hd // 2) + d // 2
+                up = d % 2
+                sc = base + ps * hd + (off * (hd // 32) + d // 32) * 2
+            code = (flat[page, byte].int() >> (4 * up).int()) & 15
+            scale = torch.stack([flat[page, sc], flat[page, sc + 1]], -1).view(torch.float16).squeeze(-1)
+            rows.append(lut[code] * scale.double())
+        got.append(torch.stack(rows))
+    return got
+
+
+def _exact_attn(s, case, q, old, new, last=None):
+    hd, g = case["hd"], case["nh"] // case["nkv"]
+    out, at = torch.zeros(q.shape, dtype=torch.float64, device=device), 0
+    for i, (a, m) in enumerate(zip(old, new)):
+        k, v = _exact_rows(s, i, a + m)
+        if last is not None:
+            k[:, a:], v[:, a:] = last[0][i][:, None], last[1][i][:, None]
+        for lo in range(0, m, 256):
+            p = torch.arange(a + lo, a + min(m, lo + 256), device=device)[:, None]
+            j = torch.arange(a + m, device=device)[None, :]
+            hide = j > p
+            if case["window"] > 0:
+                hide = hide | ((j <= p - case["window"]) & (j >= case["sink"]))
+            for h in range(case["nh"]):
+                rows = slice(at + lo, at + min(m, lo + 256))
+                w = (q[rows, h].double() / math.sqrt(hd)) @ k[h // g].T.contiguous()
+                w = torch.softmax(w.masked_fill(hide, -math.inf), -1)
+                out[rows, h] = w @ v[h // g]
+        at += m
+    return out
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    k = case["kind"]
+    if k == "plan":
+        return _exact_plan(s)
+    if k == "release":
+        return _exact_release(s)
+    if k == "append":
+        turn = _exact_turn(s.k, s, s.table, s.axis, case["halves"])
+        return {"q": _exact_turn(s.q, s, s.table, s.axis, case["halves"]), "k": _exact_held(turn), "v": _exact_held(s.v)}
+    old, new = _lens(case)
+    if k == "attn":
+        return {"out": _exact_attn(s, case, s.q, old, new)}
+    s.pos = _ints(old)
+    axis = [0] * (case["hd"] // 2)
+    held = _exact_held(_exact_turn(s.k, s, s.rope, axis, True)), _exact_held(s.v)
+    turned = _exact_turn(s.q, s, s.rope, axis, True)
+    plan = _exact_plan(s)
+    return {"q": turned, "out": _exact_attn(_State(case=case, table=plan["block_table"], pages=s.pages), case,
+                                            turned.to(DTYPE[case["dtype"]]), old, new, held),
+            "slot": plan["slot"], "kv_len": plan["kv_len"]}
