@@ -34,6 +34,31 @@ def vp(a):
     return ct.c_void_p(a.ctypes.data)
 
 
+def _struct(name, doc, ints, *rest):
+    """A ctypes structure of include/draco_hip.h: its leading ints, then (type, names) groups."""
+    fields = [(f, ct.c_int) for f in ints.split()]
+    for typ, names in rest:
+        fields += [(f, typ) for f in names.split()]
+    return type(name, (ct.Structure,), {"_fields_": fields, "__doc__": doc})
+
+
+# The paged 4-bit KV cache: device pointers (ints or None), as DracoKv4 ... in
+# include/draco_hip.h.
+_dp = ct.c_void_p
+Kv4 = type("Kv4", (ct.Structure,), {"_fields_": [("data", _dp)] + [(f, ct.c_int) for f in (
+    "n_pages", "page_size", "n_kv", "head_dim")], "__doc__": "DracoKv4: the pages of one layer"})
+KvPlan = _struct("KvPlan", "DracoKvPlan: pages for a step's new tokens", "n_seq max_blocks n_pages page_size n_tok",
+                 (_dp, "block_table kv_len q_len free_list n_free cu_q pos slot kv_len_out n_free_out status work"))
+KvRelease = _struct("KvRelease", "DracoKvRelease: pages given back", "n_seq max_blocks n_pages page_size",
+                    (_dp, "block_table block_table_out kv_len keep free_list n_free kv_len_out n_free_out work"))
+Kv4Append = _struct("Kv4Append", "DracoKv4Append: rotation and 4-bit rows", "code n_tok n_head", (_dp, "q q_out k v"),
+                    (ct.c_long, "q_stride q_out_stride k_stride v_stride"), (_dp, "slot"), (ct.c_int, "rot pairing n_axes"),
+                    (_dp, "pos"), (ct.c_long, "pos_stride"), (_dp, "table"), (ct.c_int, "table_rows"),
+                    (ct.c_uint8 * 128, "axis"))
+Kv4Attn = _struct("Kv4Attn", "DracoKv4Attn: attention of a ragged batch", "code n_seq n_tok max_q max_len n_head window sink",
+                  (ct.c_float, "scale"), (ct.c_int, "max_blocks"), (_dp, "q out"), (ct.c_long, "q_stride out_stride"),
+                  (_dp, "cu_q kv_len block_table work"), (ct.c_size_t, "work_bytes"))
+
 # name -> (restype, argtypes).  Mirrors include/draco_hip.h.
 SIGNATURES = {
     # m5 kernel-library ABI (src/m5_kern_scalar.c:146-165)
@@ -124,6 +149,14 @@ SIGNATURES = {
     "draco_gemv_q8k_f32_noalloc": (ct.c_int, [ct.c_int, ct.c_void_p, ct.c_int, ct.c_void_p, ct.c_int, ct.c_int,
                                               ct.c_void_p, ct.c_void_p]),
     "draco_noalloc_capacity": (ct.c_size_t, []),
+    # the paged 4-bit KV cache (no reference counterpart; device pointers)
+    "draco_kv4_page_bytes": (ct.c_size_t, [ct.c_int, ct.c_int, ct.c_int]),
+    "draco_kv_plan": (ct.c_int, [ct.c_void_p, ct.c_void_p]),
+    "draco_kv_release": (ct.c_int, [ct.c_void_p, ct.c_void_p]),
+    "draco_kv4_append": (ct.c_int, [ct.c_void_p, ct.c_void_p, ct.c_void_p]),
+    "draco_kv4_read": (ct.c_int, [ct.c_void_p, ct.c_void_p, ct.c_int, ct.c_void_p, ct.c_void_p, ct.c_void_p]),
+    "draco_kv4_attn_workspace": (ct.c_size_t, [ct.c_void_p, ct.c_void_p]),
+    "draco_kv4_attn": (ct.c_int, [ct.c_void_p, ct.c_void_p, ct.c_void_p]),
     "draco_quantize": (ct.c_int, [ct.c_int, f32p, ct.c_int, ct.c_int, u8p]),
     "draco_layout_query": (ct.c_size_t, [ct.c_int, ct.c_int, ct.c_int, ct.POINTER(ct.c_size_t)]),
     "draco_repack": (ct.c_int, [ct.c_int, u8p, ct.c_int, ct.c_int, u8p]),

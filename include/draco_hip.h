@@ -463,6 +463,170 @@ size_t draco_noalloc_capacity(void);
 int draco_bench_gemv_q8k(int code, const uint8_t* W, int n_out, int n_in, int nvec, int n_copies, int iters,
                          float* out);
 
+/* ---- a paged KV cache in 4 bits, for a batch of sequences -------------------
+ * No reference counterpart (its caches are one sequence's fp32 host arrays,
+ * src/m6_engine.c:396-406).  One step of a serving loop over n_seq sequences:
+ * draco_kv_plan gives the new tokens their pages, draco_kv4_append rotates q
+ * and k and writes k and v in 4 bits, draco_kv4_attn attends over the pages,
+ * draco_kv_release takes pages back.  The batch's tokens are rows [0, n_tok)
+ * of flat arrays, sequence after sequence.
+ *
+ * All array arguments are DEVICE pointers, on the device of `stream`.  Calls
+ * are enqueued on `stream` (a hipStream_t; NULL = the library's own stream, so
+ * the legacy default stream cannot be named) and not waited for.  Nothing is
+ * allocated and nothing is cleared by memset nodes: calls can be captured, and
+ * a replay reads the arrays' values of that time.  The structs are read before
+ * the call returns.  0 ok, -1 unsupported or bad argument (nothing enqueued),
+ * -2 device error.
+ *
+ * A value is code * scale: the code E2M1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a
+ * sign), one f16 scale per 32 values of a row: the largest magnitude / 6 to 9
+ * significant bits (a multiple of 2^-23, at most 10912), the code the nearest,
+ * ties to the even one.  4.5 bits per value.  Per page and KV head, in order
+ * (ps = page_size, hd = head_dim):
+ *   K codes  [ps][hd/2]         byte j: dims 2j (low nibble), 2j + 1
+ *   V codes  [ps/16][hd/2][16]  byte (16 b + a, token): dims 32 b + a (low),
+ *                               32 b + 16 + a
+ *   K scales [ps][hd/32] f16
+ *   V scales [ps/16][hd/32][16] f16
+ * Slot s is token s % ps of page s / ps. */
+typedef struct {
+    void* data;     /* n_pages * draco_kv4_page_bytes(...), 16-byte aligned */
+    int n_pages;
+    int page_size;  /* 16, 32, 64, 128 or 256 tokens */
+    int n_kv;
+    int head_dim;   /* 64, 128 or 256 */
+} DracoKv4;
+/* Bytes of a page, 0 for a shape that is not served. */
+size_t draco_kv4_page_bytes(int page_size, int n_kv, int head_dim);
+
+/* Pages for a step: sequence s holds kv_len[s] tokens in the pages of its
+ * block_table row and brings q_len[s] (0: none).  Missing pages are taken from
+ * the end of free_list[0 .. n_free), sequences and blocks in ascending order,
+ * and written into block_table.  Written: cu_q[0 .. n_seq] (the sequences'
+ * first rows), per row its position and slot (-1 for rows behind the last
+ * sequence), kv_len_out = kv_len + q_len, n_free_out.  free_list itself does
+ * not change, and kv_len_out / n_free_out may be kv_len / n_free.  A sequence
+ * whose pages are not all there (ascending order decides), or that would pass
+ * max_blocks pages or n_tok rows, is refused: its rows get position and slot
+ * -1, its length and pages stay, later ones are still served where they need
+ * no page or enough are left of the count before the refused.  status[0] =
+ * sequences refused, status[1] = rows beyond n_tok.  Negative lengths count
+ * as 0.  `work`: one int, 0 before its first use and left 0; calls that
+ * overlap need their own. */
+typedef struct {
+    int n_seq, max_blocks, n_pages, page_size, n_tok;
+    int* block_table;      /* [n_seq][max_blocks], in / out */
+    const int* kv_len;     /* [n_seq] */
+    const int* q_len;      /* [n_seq] */
+    const int* free_list;  /* [n_pages] */
+    const int* n_free;     /* [1] */
+    int* cu_q;             /* [n_seq + 1] */
+    int* pos;              /* [n_tok] (nullable) */
+    int* slot;             /* [n_tok] */
+    int* kv_len_out;       /* [n_seq] */
+    int* n_free_out;       /* [1] */
+    int* status;           /* [2] */
+    int* work;             /* [1] */
+} DracoKvPlan;
+int draco_kv_plan(const DracoKvPlan* p, void* stream);
+
+/* Pages given back: sequence s keeps its first min(keep[s], kv_len[s]) tokens
+ * (0: it ended; less than it holds: drafted tokens taken back).  Pages behind
+ * them go onto free_list and leave -1 in block_table_out (other entries are
+ * not written; it may be block_table), in the reverse of a plan's order: a
+ * release of what a plan just took restores the list.  kv_len_out = the tokens
+ * kept, n_free_out the list's new count; they may be kv_len / n_free.  `work`
+ * as in draco_kv_plan. */
+typedef struct {
+    int n_seq, max_blocks, n_pages, page_size;
+    const int* block_table;
+    int* block_table_out;
+    const int* kv_len;
+    const int* keep;       /* [n_seq] */
+    int* free_list;        /* [n_pages], in / out */
+    const int* n_free;
+    int* kv_len_out;
+    int* n_free_out;
+    int* work;             /* [1] */
+} DracoKvRelease;
+int draco_kv_release(const DracoKvRelease* p, void* stream);
+
+/* n_tok rows: q rotated into q_out, k rotated and v as they are written into
+ * their slots in 4 bits.  A row whose slot is negative or past the pool is
+ * skipped whole (its q_out too).  Two rows of one call must not share a slot.
+ * code: the rows' type, 9 F32 or 7 F16; strides in elements per token,
+ * multiples of 8, rows 16-byte aligned, heads of head_dim next to each other.
+ * n_head 0: no q.
+ *
+ * Rotation of the first `rot` dims of every head (a multiple of 8; 0: none):
+ * pair i is (2i, 2i + 1) with pairing 0, (i, i + rot/2) with pairing 1, and
+ * turns by row pos[axis[i]][token] of `table` ([table_rows][rot/2] of cos,
+ * sin: draco_rope_table's layout).  Text has one axis; images and video up to
+ * four (time, height, width, ...), each with its own positions, pos_stride
+ * ints apart.  Products and sums in 64 bits, one rounding.  A position outside
+ * the table makes its pairs NaN.  q_out may be q with pairing 0 or rot 0 only.
+ *
+ * A k or v row that is not finite is held as NaN: attention rows that see the
+ * token become NaN, others do not.  Magnitudes past 65472 saturate. */
+typedef struct {
+    int code;
+    int n_tok, n_head;
+    const void* q;
+    void* q_out;
+    const void* k;
+    const void* v;
+    long q_stride, q_out_stride, k_stride, v_stride;
+    const int* slot;       /* [n_tok] */
+    int rot, pairing, n_axes;
+    const int* pos;        /* [n_axes][pos_stride] */
+    long pos_stride;
+    const float* table;
+    int table_rows;
+    uint8_t axis[128];     /* axis of pair i < rot / 2 */
+} DracoKv4Append;
+int draco_kv4_append(const DracoKv4* cache, const DracoKv4Append* p, void* stream);
+
+/* The values of n slots as fp32 rows k, v [n][n_kv][head_dim] (a snapshot);
+ * rows of slots outside the pool are not written. */
+int draco_kv4_read(const DracoKv4* cache, const int* slot, int n, float* k, float* v, void* stream);
+
+/* Causal attention of the batch's rows over the pages: sequence s has
+ * cu_q[s + 1] - cu_q[s] rows, the last of its kv_len[s] cached tokens (so a
+ * step appends first, and kv_len is the plan's kv_len_out).  A row at position
+ * p sees keys j <= p with j > p - window (window 0: all) or j < sink (the
+ * first tokens, which stay visible).  scale: of the scores (1 / sqrt(head_dim)
+ * as a rule), in 1e-12 .. 1e12.  Rows that see nothing give 0; rows of no
+ * sequence are left as they are.  n_head a multiple of n_kv; q and out as in
+ * draco_kv4_append (out must not be q).  One call serves decode (one row a
+ * sequence), drafts and prompt chunks, mixed as they come.
+ *
+ * max_q, max_len: the largest row count and length of a sequence, or more;
+ * smaller values only cost speed.  A length past max_blocks pages, or a page
+ * outside the pool that a row sees, gives NaN.  work / work_bytes: at least
+ * draco_kv4_attn_workspace(cache, p) bytes (it reads sizes only), 16-byte
+ * aligned, any content; calls that overlap need their own.  Results do not
+ * depend on the other rows of the batch's values, and a call's are the same
+ * every time. */
+typedef struct {
+    int code;
+    int n_seq, n_tok, max_q, max_len;
+    int n_head;
+    int window, sink;
+    float scale;
+    int max_blocks;
+    const void* q;
+    void* out;
+    long q_stride, out_stride;
+    const int* cu_q;         /* [n_seq + 1] */
+    const int* kv_len;       /* [n_seq] */
+    const int* block_table;  /* [n_seq][max_blocks] */
+    void* work;
+    size_t work_bytes;
+} DracoKv4Attn;
+size_t draco_kv4_attn_workspace(const DracoKv4* cache, const DracoKv4Attn* p);
+int draco_kv4_attn(const DracoKv4* cache, const DracoKv4Attn* p, void* stream);
+
 /* Device timing probes (weights rotated over n_copies device copies so the
  * working set can exceed the 256 MB MALL).  out[0] mean us per launch from
  * per-launch event pairs, out[1] us per launch over the whole loop, out[2]
