@@ -55,6 +55,7 @@ int cus_of(int device) {
     if (!n[device]) {
         int v = 0;
         if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || v < 1) v = 256;
+        if (v > KV4_MAX_BLOCKS / 4) v = KV4_MAX_BLOCKS / 4;
         n[device] = v;
     }
     return n[device];
@@ -73,7 +74,7 @@ int view_of(const DracoKv4* c, Kv4View* v, const char* who) {
     if (!aligned(c->data, 16)) return fail(-1, "%s: the pages are not 16-byte aligned", who);
     v->data = (uint8_t*)c->data;
     v->head_bytes = (int)kv4_head_bytes(c->page_size, c->head_dim);
-    v->page_bytes = (long)v->head_bytes * c->n_kv;
+    v->page_bytes = (unsigned)v->head_bytes * (unsigned)c->n_kv;
     v->n_pages = c->n_pages;
     v->ps_shift = __builtin_ctz((unsigned)c->page_size);
     v->n_kv = c->n_kv;
@@ -122,7 +123,7 @@ int attn_args(const DracoKv4* cache, const DracoKv4Attn* p, Kv4AttnArgs* a, bool
     if (int rc = type_of(p->code, f16, who)) return rc;
     if (int rc = heads_ok(p->n_head, cache->n_kv, who)) return rc;
     if (int rc = batch_ok(p->n_seq, p->max_blocks, cache->n_pages, cache->page_size, who)) return rc;
-    if (p->n_tok < 0) return fail(-1, "%s: n_tok %d", who, p->n_tok);
+    if (p->n_tok < 0 || (long)p->n_tok * p->n_head > 0x7FFFFFFFL) return fail(-1, "%s: n_tok %d", who, p->n_tok);
     if (p->n_tok > 0 && p->n_seq > 0 && (p->max_q < 1 || p->max_len < 0))
         return fail(-1, "%s: max_q %d, max_len %d", who, p->max_q, p->max_len);
     if (p->window < 0 || p->sink < 0) return fail(-1, "%s: window %d, sink %d", who, p->window, p->sink);
@@ -131,9 +132,7 @@ int attn_args(const DracoKv4* cache, const DracoKv4Attn* p, Kv4AttnArgs* a, bool
 }
 
 Kv4AttnPlan plan_of(const DracoKv4* c, const DracoKv4Attn* p, bool f16, int cus) {
-    const int max_q = p->max_q < p->n_tok ? p->max_q : p->n_tok;
-    const long cap = (long)p->max_blocks * c->page_size, len = p->max_len < cap ? p->max_len : cap;
-    return kv4_attn_plan(c->head_dim, f16, p->n_seq, p->n_tok, p->n_head, c->n_kv, max_q, len, p->window, p->sink, cus);
+    return kv4_attn_plan(c->head_dim, f16, p->n_seq, p->n_tok, p->n_head, c->n_kv, p->max_q < p->n_tok ? p->max_q : p->n_tok, cus);
 }
 
 }  // namespace
@@ -297,8 +296,7 @@ int draco_kv4_attn(const DracoKv4* cache, const DracoKv4Attn* p, void* stream) {
     a.window = p->window;
     a.sink = p->sink;
     a.scale_log2 = (float)((double)p->scale * 1.4426950408889634);
-    a.part = (float*)p->work;
-    return launched(kv4_attn(a, f16, plan, st), who);
+    return launched(kv4_attn(a, f16, plan, p->work, st), who);
 }
 
 }  // extern "C"

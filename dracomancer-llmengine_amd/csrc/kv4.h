@@ -25,7 +25,7 @@ namespace draco {
 
 struct Kv4View {
     uint8_t* data;
-    long page_bytes;  // n_kv * head_bytes
+    unsigned page_bytes;  // n_kv * head_bytes (4096 heads of 256 tokens of 256 dims: 302 MB at most)
     int head_bytes;   // ps * (hd + hd / 8)
     int n_pages, ps_shift, n_kv, hd;
 };
@@ -58,18 +58,23 @@ struct Kv4AttnArgs {
     int n_seq, n_tok, n_head, group, max_blocks;
     int window, sink;
     float scale_log2;  // scale * log2(e)
-    int tiles;         // row tiles per (sequence, kv head)
-    int n_split;
-    float* part;       // n_split > 1: [n_tok * n_head][n_split] rows of hd + 4 floats
+    int chunk;           // units of 64 keys a block takes at least
+    int* count;          // per block: of the tile that it leaves unfinished, blocks that are done; 0 between calls
+    float* part;         // two slots a block: [rows of a tile][hd + 4]
+    unsigned part_bytes;
+    bool whole;          // a tile per block instead (no counters, no partial rows)
 };
+constexpr int KV4_MAX_BLOCKS = 4096;
+constexpr size_t KV4_COUNT_BYTES = KV4_MAX_BLOCKS * sizeof(int);
 struct Kv4AttnPlan {
-    int tiles, rows, n_split;
-    bool shared;   // the chunk kernel (K / V tiles shared by a block's waves)
-    size_t work;   // bytes of workspace
+    int rows;            // of a tile: 16 (decode), else the chunk kernel's
+    bool whole;
+    long grid;
+    int chunk;
+    size_t part_bytes, work;  // bytes of partial rows, of workspace
 };
-Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, long max_len,
-                          int window, int sink, int cus);
-int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, hipStream_t st);
+Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, int cus);
+int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, void* work, hipStream_t st);
 
 struct KvPlanArgs {
     int n_seq, max_blocks, n_pages, ps_shift, n_tok;

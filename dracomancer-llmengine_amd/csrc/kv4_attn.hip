@@ -52,21 +52,6 @@ __device__ __forceinline__ h8v k_operand(uint32_t w, h2v s) {
 __device__ __forceinline__ h2v as_h2(uint32_t u) { return __builtin_bit_cast(h2v, u); }
 __device__ __forceinline__ uint32_t as_u(h2v h) { return __builtin_bit_cast(uint32_t, h); }
 
-// Eight consecutive tokens' bytes (w0, w1) of a pair of dims, times the
-// tokens' scales: the operand of the low nibbles' dim and of the high ones'.
-__device__ __forceinline__ void v_operands(uint32_t w0, uint32_t w1, const uint32_t s[4], h8v& lo, h8v& hi) {
-    uint32_t l[4], h[4];
-    const h2v c[8] = {fp4x2<0>(w0), fp4x2<1>(w0), fp4x2<2>(w0), fp4x2<3>(w0),
-                      fp4x2<0>(w1), fp4x2<1>(w1), fp4x2<2>(w1), fp4x2<3>(w1)};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        l[i] = as_u(as_h2(__builtin_amdgcn_perm(as_u(c[2 * i + 1]), as_u(c[2 * i]), 0x05040100)) * as_h2(s[i]));
-        h[i] = as_u(as_h2(__builtin_amdgcn_perm(as_u(c[2 * i + 1]), as_u(c[2 * i]), 0x07060302)) * as_h2(s[i]));
-    }
-    lo = __builtin_bit_cast(h8v, u4v{l[0], l[1], l[2], l[3]});
-    hi = __builtin_bit_cast(h8v, u4v{h[0], h[1], h[2], h[3]});
-}
-
 // Eight fp32 values as one (F16) or two f16 operands.
 template <bool F16>
 __device__ __forceinline__ void split8(const float x[8], h8v& hi, h8v& lo) {
@@ -78,11 +63,12 @@ __device__ __forceinline__ void split8(const float x[8], h8v& hi, h8v& lo) {
     }
 }
 
-// What a block works on: one sequence's rows [r0, r0 + rows) of a KV head.
+// Rows [r0, r1) of one sequence and KV head.
 struct Tile {
-    int q0, qn, len, rows, r0, head;  // head: the KV head
-    bool bad;                         // the length passes the table: NaN
-    long pos0;                        // position of the sequence's first query
+    int seq, q0, rows, len, r0, r1, head;  // rows: of the whole sequence; head: the KV head
+    bool bad;                              // the length passes the table: NaN
+    long pos0;                             // position of the sequence's first query
+    const int* table;
 };
 
 // The KV rows that the tile's queries can see, as units of 64: first the sink
@@ -101,100 +87,273 @@ __device__ __forceinline__ Units units_of(long first_pos, long last_pos, int win
     return u;
 }
 
-__device__ __forceinline__ void seq_of(const Kv4AttnArgs& a, int seq, int head, Tile& t) {
-    t.q0 = min(max(a.cu_q[seq], 0), a.n_tok);
-    t.qn = min(max(a.cu_q[seq + 1], t.q0), a.n_tok) - t.q0;
-    t.rows = t.qn * a.group;
-    t.head = head;
-    const int len = max(a.kv_len[seq], 0);
-    const long cap = (long)a.max_blocks << a.c.ps_shift;
-    t.bad = len > cap;
-    t.len = t.bad ? 0 : len;
-    t.pos0 = (long)t.len - t.qn;
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long uni(long v) {
+    return (long)((unsigned long)(unsigned)uni((int)v) | (unsigned long)(unsigned)uni((int)(v >> 32)) << 32);
 }
 
-// Address of a page's head, or null for a page outside the pool.
-__device__ __forceinline__ const uint8_t* page_ptr(const Kv4AttnArgs& a, const int* table, int key, int head) {
-    const int b = key >> a.c.ps_shift;
-    const int p = b < a.max_blocks ? table[b] : 0;  // past the table only behind the last key
-    return (unsigned)p < (unsigned)a.c.n_pages ? a.c.data + (long)p * a.c.page_bytes + (long)head * a.c.head_bytes : nullptr;
+// 64 sequences' rows and lengths, one a lane.
+struct Batch {
+    int base, q0, q1, len;
+};
+__device__ __forceinline__ void batch_of(const Kv4AttnArgs& a, int base, Batch& b) {
+    const int s = min(base + ((int)threadIdx.x & 63), a.n_seq - 1);
+    b.base = base;
+    b.q0 = a.cu_q[s];
+    b.q1 = a.cu_q[s + 1];
+    b.len = a.kv_len[s];
+}
+__device__ __forceinline__ void tile_of(const Kv4AttnArgs& a, int q0, int q1, int len, Tile& t) {
+    t.q0 = min(max(q0, 0), a.n_tok);
+    const int qn = min(max(q1, t.q0), a.n_tok) - t.q0;
+    t.rows = qn * a.group;
+    t.bad = len > (long)a.max_blocks << a.c.ps_shift;
+    t.len = t.bad ? 0 : max(len, 0);
+    t.pos0 = (long)t.len - qn;
+}
+__device__ __forceinline__ void seq_of(const Kv4AttnArgs& a, Batch& b, int seq, Tile& t) {
+    if (seq >= b.base + 64) batch_of(a, seq, b);
+    const int l = seq - b.base;
+    tile_of(a, __builtin_amdgcn_readlane(b.q0, l), __builtin_amdgcn_readlane(b.q1, l), __builtin_amdgcn_readlane(b.len, l), t);
+    t.seq = seq;
+    t.table = a.block_table + (long)seq * a.max_blocks;
+}
+__device__ __forceinline__ Units tile_units(const Kv4AttnArgs& a, const Tile& t, int r0, int r1) {
+    return units_of(t.pos0 + r0 / a.group, t.pos0 + (r1 - 1) / a.group, a.window, a.sink);
 }
 
-template <int HD>
-struct KRaw {  // one wave's K of a unit
-    static constexpr int W = HD / 32;  // 8-code words per lane and tile
-    uint32_t w[4][W];
-    uint16_t s[4][HD == 256 ? 2 : 1];
+// The batch's work, laid out as one list of units: sequences, their tiles of R
+// rows, KV heads, units of keys (at least one each, so that every row is
+// written).  The grid's blocks take equal stretches of it, whatever the
+// lengths are: `chunk` units from `at`.  Lengths come from device memory, so
+// every wave adds them up itself, 64 sequences at a time.
+struct Work {
+    long at;      // this block's next unit
+    int left;     // units left to it
+    int chunk;
+    long rem;     // `at` within sequence `seq`
+    int seq;
 };
-template <int HD>
-struct VRaw {
-    static constexpr int B = HD / 32;
-    u4v w[B], s[B][2];
+// Units of this lane's sequence.
+template <int R>
+__device__ __forceinline__ long batch_units(const Kv4AttnArgs& a, const Batch& b) {
+    if (b.base + ((int)threadIdx.x & 63) >= a.n_seq) return 0;
+    Tile t;
+    tile_of(a, b.q0, b.q1, b.len, t);
+    long n = 0;
+    for (int r = 0; r < t.rows; r += R) n += max(tile_units(a, t, r, min(r + R, t.rows)).n, 1);
+    return n * a.c.n_kv;
+}
+// Inclusive sums over the lanes, and lane l's value.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long dpp_up(long v) {  // 0 where no lane lies that far back
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (long)((unsigned long)(unsigned)lo | (unsigned long)(unsigned)hi << 32);
+}
+__device__ __forceinline__ long wave_scan(long v) {
+    v += dpp_up<0x111, 0xF>(v);  // within rows of 16: 1, 2, 4 and 8 lanes back
+    v += dpp_up<0x112, 0xF>(v);
+    v += dpp_up<0x114, 0xF>(v);
+    v += dpp_up<0x118, 0xF>(v);
+    v += dpp_up<0x142, 0xA>(v);  // a row's last lane to the next row, then lane 31 to the upper half
+    v += dpp_up<0x143, 0xC>(v);
+    return v;
+}
+__device__ __forceinline__ long lane_of(long v, int l) {
+    return (long)((unsigned long)(unsigned)__builtin_amdgcn_readlane((int)v, l) |
+                  (unsigned long)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32);
+}
+template <int R>
+__device__ __forceinline__ bool work_of(const Kv4AttnArgs& a, Work& w, Batch& b) {
+    batch_of(a, 0, b);
+    long mine = wave_scan(batch_units<R>(a, b)), total = lane_of(mine, 63);
+    for (int s = 64; s < a.n_seq; s += 64) {
+        batch_of(a, s, b);
+        total += lane_of(wave_scan(batch_units<R>(a, b)), 63);
+    }
+    w.chunk = max(a.chunk, (int)((total + gridDim.x - 1) / gridDim.x));
+    w.at = (long)blockIdx.x * w.chunk;
+    w.left = (int)min((long)w.chunk, total - w.at);
+    if (w.left <= 0) return false;
+    long before = 0;
+    for (int s = 0;; s += 64) {
+        if (a.n_seq > 64) {
+            batch_of(a, s, b);
+            mine = wave_scan(batch_units<R>(a, b));
+        }
+        const unsigned long long past = __ballot(before + mine > w.at);
+        if (past) {
+            const int l = uni(__ffsll((long long)past) - 1);
+            w.seq = s + l;
+            w.rem = w.at - before - (l ? lane_of(mine, l - 1) : 0L);
+            return true;
+        }
+        before += lane_of(mine, 63);
+    }
+}
+
+// One tile a block, whole (prompts: enough of them, and partial rows of many
+// queries cost more than they balance).  A sequence's tiles start at v(s) =
+// floor(cu_q[s] * group / R) + s, which leaves it at least ceil(rows / R) of
+// them; the wave looks for the last s with v(s) <= id, 64 at a time.  The last
+// rows (the most keys) come first.
+template <int R>
+__device__ __forceinline__ bool whole_tile(const Kv4AttnArgs& a, Tile& t) {
+    const int lane = threadIdx.x & 63;
+    t.head = blockIdx.x % a.c.n_kv;  // neighbours on other XCDs: a head's tiles share few L2s
+    const int id = blockIdx.x / a.c.n_kv;
+    auto start = [&](int s) { return (int)((long)min(max(a.cu_q[s], 0), a.n_tok) * a.group / R) + s; };
+    int seq = 0;
+    for (int stride = a.n_seq; stride > 1;) {
+        const int end = min(seq + stride, a.n_seq);
+        stride = (stride + 63) / 64;
+        const int s = seq + lane * stride;
+        const bool in = s < end && start(s) <= id;
+        seq += max((int)__popcll(__ballot(in)) - 1, 0) * stride;
+    }
+    t.seq = seq = uni(seq);
+    t.table = a.block_table + (long)seq * a.max_blocks;
+    tile_of(a, a.cu_q[seq], a.cu_q[seq + 1], a.kv_len[seq], t);
+    const int n = (t.rows + R - 1) / R, k = n - 1 - (id - start(seq));
+    if (k < 0 || k >= n) return false;
+    t.r0 = k * R;
+    t.r1 = min(t.r0 + R, t.rows);
+    return true;
+}
+
+// The next piece of a block's work: units [lo, hi) of u for a tile.
+struct Piece {
+    int lo, hi;
+    long first;  // the tile's first unit in the list
+    int n;       // its units there
 };
+template <int R>
+__device__ __forceinline__ void piece_of(const Kv4AttnArgs& a, Work& w, Batch& b, Tile& t, Units& u, Piece& p) {
+    for (;;) {
+        seq_of(a, b, w.seq, t);
+        long rem = w.rem;
+        for (t.r0 = 0; t.r0 < t.rows; t.r0 += R) {
+            t.r1 = min(t.r0 + R, t.rows);
+            u = tile_units(a, t, t.r0, t.r1);
+            p.n = max(u.n, 1);
+            if (rem < (long)p.n * a.c.n_kv) {
+                for (t.head = 0; rem >= p.n; t.head++) rem -= p.n;
+                p.lo = (int)rem;
+                p.hi = min(p.lo + w.left, p.n);
+                p.first = w.at - p.lo;
+                const int took = p.hi - p.lo;
+                w.at += took;
+                w.rem += took;
+                w.left -= took;
+                p.hi = min(p.hi, u.n);
+                return;
+            }
+            rem -= (long)p.n * a.c.n_kv;
+        }
+        w.rem = rem;
+        w.seq++;  // (its rows are done; `left` says that more follow)
+    }
+}
+
+// The table's page that holds `key` (an entry past the table, which only keys
+// behind the last one have, is not read: `page_ptr` refuses it).  The loads of
+// a unit are issued a turn before their use: nothing here may look at what
+// they bring, or the wave would wait for it at once.
+__device__ __forceinline__ int page_of(const Kv4AttnArgs& a, const int* table, int key) {
+    return table[min(key >> a.c.ps_shift, a.max_blocks - 1)];
+}
+// The page's part of a head; a page outside the pool gives any readable one and ok = false.
+__device__ __forceinline__ const uint8_t* page_ptr(const Kv4AttnArgs& a, int page, int key, int head, bool& ok) {
+    ok = (unsigned)page < (unsigned)a.c.n_pages && key >> a.c.ps_shift < a.max_blocks;
+    return a.c.data + (unsigned long)(ok ? (unsigned)page : 0u) * a.c.page_bytes + (unsigned long)(unsigned)head * (unsigned)a.c.head_bytes;
+}
 
 // Lane (i = lane & 15, g = lane >> 4) of operand tile t holds dims of key
 // 16 (i / 4) + 4 t + i % 4: tile t's result rows are then keys 16 g' + 4 t + r
 // for lane group g', so that a lane group ends with 16 consecutive keys.
-template <int HD>
-__device__ __forceinline__ void load_k(const Kv4AttnArgs& a, const int* table, int head, int unit, KRaw<HD>& k) {
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int ps = 1 << a.c.ps_shift;
-    const int key = unit * UNIT + 16 * (i >> 2) + (i & 3);
-    const uint8_t* p = page_ptr(a, table, key, head);
-    const bool ok = p != nullptr;
-    if (!ok) p = a.c.data;  // any readable page; its scores become NaN
-    const int off = key & (ps - 1);
-    const uint8_t* sc = p + ps * HD;
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        const uint8_t* row = p + (off + 4 * t) * (HD / 2);
-        if constexpr (HD == 64) {
-            const u2v v = *gptr<u2v>(row + g * 8);
-            k.w[t][0] = v.x, k.w[t][1] = v.y;
-            k.s[t][0] = *gptr<uint16_t>(sc + ((off + 4 * t) * 2 + (g >> 1)) * 2);
-        } else {
-#pragma unroll
-            for (int c = 0; c < HD / 128; c++) {
-                const u4v v = *gptr<u4v>(row + c * 64 + g * 16);
-                k.w[t][4 * c] = v.x, k.w[t][4 * c + 1] = v.y, k.w[t][4 * c + 2] = v.z, k.w[t][4 * c + 3] = v.w;
-                k.s[t][c] = *gptr<uint16_t>(sc + ((off + 4 * t) * (HD / 32) + c * 4 + g) * 2);
-            }
-        }
-        if (!ok) k.s[t][0] = 0x7E00;
+__device__ __forceinline__ int k_key(int unit) {
+    const int i = threadIdx.x & 15;
+    return unit * UNIT + 16 * (i >> 2) + (i & 3);
+}
+__device__ __forceinline__ int v_key(int unit) { return unit * UNIT + 16 * ((threadIdx.x & 63) >> 4); }
+
+// N words of 8 codes of one K row and their block scales.  Word s of a row (s =
+// 0 .. HD / 32 - 1 in a lane) holds dims HD == 64: 16 g + 8 s; else
+// 128 (s / 4) + 32 g + 8 (s % 4).
+template <int HD, int N>
+struct KRow {
+    uint32_t w[N];
+    uint16_t s[N > 4 ? 2 : 1];
+    bool ok;
+    // Scale of word j for both halves; NaN for a page that is none.
+    __device__ __forceinline__ h2v scale(int j) const {
+        const uint32_t x = ok ? s[N > 4 ? j >> 2 : 0] : 0x7E00u;
+        return as_h2(x | x << 16);
     }
+};
+template <int HD, int N>
+__device__ __forceinline__ void load_krow(const uint8_t* p, bool ok, int ps, int off, int s0, KRow<HD, N>& k) {
+    const int g = (threadIdx.x & 63) >> 4;
+    const uint8_t* sc = p + ps * HD;
+    const uint8_t* row = p + off * (HD / 2) + (HD == 64 ? g * 8 + s0 * 4 : (s0 >> 2) * 64 + g * 16 + (s0 & 3) * 4);
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int c = 0; c < N / 4; c++) {
+            const u4v v = *gptr<u4v>(row + c * 64);
+            k.w[4 * c] = v.x, k.w[4 * c + 1] = v.y, k.w[4 * c + 2] = v.z, k.w[4 * c + 3] = v.w;
+        }
+    } else if constexpr (N == 2) {
+        const u2v v = *gptr<u2v>(row);
+        k.w[0] = v.x, k.w[1] = v.y;
+    } else {
+        k.w[0] = *gptr<uint32_t>(row);
+    }
+#pragma unroll
+    for (int c = 0; c < (N > 4 ? 2 : 1); c++) {
+        const int blk = HD == 64 ? g >> 1 : ((s0 >> 2) + c) * 4 + g;
+        k.s[c] = *gptr<uint16_t>(sc + (off * (HD / 32) + blk) * 2);
+    }
+    k.ok = ok;
 }
 
-// Lane (i, g): bytes of 16 tokens (the page group of keys 16 g ..) for dims
-// 32 b + i and 32 b + 16 + i.
+// Eight tokens (half x of the lane group's 16) of dims 32 b + i and 32 b + 16 + i.
+struct VPart {
+    u2v w;
+    u4v s;
+};
 template <int HD>
-__device__ __forceinline__ void load_v(const Kv4AttnArgs& a, const int* table, int head, int unit, int len, VRaw<HD>& v) {
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int ps = 1 << a.c.ps_shift;
-    const int key = unit * UNIT + 16 * g;
-    const uint8_t* p = page_ptr(a, table, key, head);
-    const bool ok = p != nullptr && key < len;
-    if (p == nullptr) p = a.c.data;
-    const int grp = (key & (ps - 1)) >> 4;
-    const uint8_t* w = p + ps * (HD / 2) + grp * (HD * 8) + i * 16;
-    const uint8_t* s = p + ps * HD + ps * (HD / 16) + grp * HD;
+__device__ __forceinline__ void load_vpart(const uint8_t* p, int ps, int off, int b, int x, VPart& v) {
+    const int i = threadIdx.x & 15, grp = off >> 4;
+    v.w = *gptr<u2v>(p + ps * (HD / 2) + grp * (HD * 8) + (b * 16 + i) * 16 + x * 8);
+    v.s = *gptr<u4v>(p + ps * HD + ps * (HD / 16) + grp * HD + b * 32 + x * 16);
+}
+// The part's values: the operand of the low nibbles' dim and of the high ones'.
+__device__ __forceinline__ void v_operands(const VPart& v, h8v& lo, h8v& hi) {
+    const uint32_t w0 = v.w.x, w1 = v.w.y;
+    uint32_t l[4], h[4];
+    const h2v c[8] = {fp4x2<0>(w0), fp4x2<1>(w0), fp4x2<2>(w0), fp4x2<3>(w0),
+                      fp4x2<0>(w1), fp4x2<1>(w1), fp4x2<2>(w1), fp4x2<3>(w1)};
 #pragma unroll
-    for (int b = 0; b < HD / 32; b++) {
-        v.w[b] = *gptr<u4v>(w + b * 256);
-        v.s[b][0] = *gptr<u4v>(s + b * 32);
-        v.s[b][1] = *gptr<u4v>(s + b * 32 + 16);
+    for (int i = 0; i < 4; i++) {
+        l[i] = as_u(as_h2(__builtin_amdgcn_perm(as_u(c[2 * i + 1]), as_u(c[2 * i]), 0x05040100)) * as_h2(v.s[i]));
+        h[i] = as_u(as_h2(__builtin_amdgcn_perm(as_u(c[2 * i + 1]), as_u(c[2 * i]), 0x07060302)) * as_h2(v.s[i]));
     }
-    // Rows behind the last token hold anything, NaN scales too: p = 0 would not
-    // hide them.  (A row that is in the cache has finite V scales.)
-    if (unit * UNIT + UNIT > len || !ok) {
+    lo = __builtin_bit_cast(h8v, u4v{l[0], l[1], l[2], l[3]});
+    hi = __builtin_bit_cast(h8v, u4v{h[0], h[1], h[2], h[3]});
+}
+
+// Rows behind the last token hold anything, NaN scales too: p = 0 would not
+// hide them.  (A row that is in the cache has finite V scales.)  key: the
+// part's first; n: keys that are there.
+__device__ __forceinline__ void cut_vpart(VPart& v, int key, int len) {
 #pragma unroll
-        for (int b = 0; b < HD / 32; b++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                uint32_t x = v.s[b][e >> 2][e & 3];
-                if (!ok || key + 2 * e >= len) x = 0;
-                else if (key + 2 * e + 1 >= len) x &= 0xFFFFu;
-                v.s[b][e >> 2][e & 3] = x;
-            }
+    for (int e = 0; e < 4; e++) {
+        uint32_t s = v.s[e];
+        if (key + 2 * e >= len) s = 0;
+        else if (key + 2 * e + 1 >= len) s &= 0xFFFFu;
+        v.s[e] = s;
     }
 }
 
@@ -237,23 +396,6 @@ __device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const Tile& t, int 
     }
 }
 
-// Scores of a unit against a 16-row tile: c[t][r] for key 16 g + 4 t + r.
-template <int HD, bool F16>
-__device__ __forceinline__ void scores(const KRaw<HD>& k, const h8v* hi, const h8v* lo, f4v c[4]) {
-    constexpr int KS = HD / 32;
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        c[t] = f4v{0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const uint32_t sc = k.s[t][HD == 256 ? s >> 2 : 0];
-            const h8v w = k_operand(k.w[t][s], as_h2(sc | sc << 16));
-            c[t] = mfma(w, hi[s], c[t]);
-            if constexpr (!F16) c[t] = mfma(w, lo[s], c[t]);
-        }
-    }
-}
-
 // Softmax state of a lane's query row.
 struct Row {
     int pos, lo;    // keys j <= pos, and j >= lo or j < sink
@@ -272,9 +414,18 @@ __device__ __forceinline__ void row_init(const Kv4AttnArgs& a, const Tile& t, in
     w.l = t.bad ? __builtin_nanf("") : 0.0f;
 }
 
+// Keys that every one of rows [r0, r1) sees: [lo, hi].
+struct Whole {
+    int lo, hi;
+    __device__ __forceinline__ bool has(int key0) const { return key0 >= lo && key0 + UNIT - 1 <= hi; }
+};
+__device__ __forceinline__ Whole whole_of(const Kv4AttnArgs& a, const Tile& t, int r0, int r1) {
+    return {a.window > 0 ? (int)max(0L, t.pos0 + (r1 - 1) / a.group - a.window + 1) : 0, (int)(t.pos0 + r0 / a.group)};
+}
+
 template <bool MASK>
-__device__ __forceinline__ bool row_max(const Row& w, int key, int sink, f4v c[4], float& top) {
-    top = -__builtin_inff();
+__device__ __forceinline__ float row_max(const Row& w, int key, int sink, f4v c[4]) {
+    float top = -__builtin_inff();
 #pragma unroll
     for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -286,49 +437,39 @@ __device__ __forceinline__ bool row_max(const Row& w, int key, int sink, f4v c[4
             }
             top = fmaxf(top, c[t][r]);
         }
-    top = rows_reduce(top, OpMax{});
-    return top > w.m && !(w.f * (top - w.m) <= PSLACK);
+    return rows_reduce(top, OpMax{});
 }
 
-// A block's four waves hold the same rows over different keys: their sums to
-// one.  acc[m]: O^T tiles, dims 16 m + 4 g + r of row i.  Wave w ends with the
-// tiles m = 4 c + w of every chunk c, in out[c].
-template <int HD>
-__device__ __forceinline__ void join_waves(f4v* acc, float nfm, float& l, float* nfm_all, float* smem, f4v* out) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15;
-    l = rows_sum(l);
-    float* s_n = smem;        // [4][16]
-    float* s_l = smem + 64;   // [4][16]
-    f4v* s_o = (f4v*)(smem + 128);  // [4 waves][4 tiles][64 lanes]
-    __syncthreads();
-    if (lane < 16) {
-        s_n[wave * 16 + i] = l != 0.0f ? nfm : __builtin_inff();  // no key seen: no weight (NaN counts as seen)
-        s_l[wave * 16 + i] = l;
+// Scores c (keys 16 g + 4 t + r of the unit at key0) to probabilities as the
+// second product's operands; acc follows the reference score where it moves.
+// The reference moves only when a maximum passes it by 2^PSLACK, so that most
+// units leave acc alone.
+template <bool F16, int MT>
+__device__ __forceinline__ void softmax(Row& w, bool whole, int key0, int sink, f4v c[4], f4v* acc, h8v ph[2], h8v pl[2]) {
+    const int key = key0 + 16 * ((threadIdx.x & 63) >> 4);
+    const float top = whole ? row_max<false>(w, key, sink, c) : row_max<true>(w, key, sink, c);
+    const bool grow = top > w.m && !(w.f * (top - w.m) <= PSLACK);
+    if (__any(grow)) {
+        const float nfm = grow ? PBIAS - w.f * top : w.nfm;
+        const float keep = !grow ? 1.0f : w.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(nfm - w.nfm);
+        if (grow) w.m = top;
+        w.nfm = nfm;
+        w.l *= keep;
+#pragma unroll
+        for (int m = 0; m < MT; m++) acc[m] *= keep;
     }
-    __syncthreads();
-    float n = s_n[i];
+    float p[2][8], sum = 0.0f;
 #pragma unroll
-    for (int w = 1; w < 4; w++) n = fminf(n, s_n[w * 16 + i]);
-    float sum = 0.0f;
+    for (int x = 0; x < 4; x++)
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const float x = s_l[w * 16 + i];
-        if (x != 0.0f) sum += x * exp2f(n - s_n[w * 16 + i]);
-    }
-    const float mine = l != 0.0f ? exp2f(n - nfm) : 0.0f;
-    l = sum;
-    *nfm_all = n;
-#pragma unroll
-    for (int c = 0; c < HD / 64; c++) {
-#pragma unroll
-        for (int m = 0; m < 4; m++) s_o[(wave * 4 + m) * 64 + lane] = acc[4 * c + m] * mine;
-        __syncthreads();
-        f4v o = s_o[wave * 64 + lane];
-#pragma unroll
-        for (int w = 1; w < 4; w++) o += s_o[(w * 4 + wave) * 64 + lane];
-        out[c] = o;
-        __syncthreads();
-    }
+        for (int y = 0; y < 4; y++) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y], w.f, w.nfm));
+            p[x >> 1][(x & 1) * 4 + y] = e;
+            sum += e;
+        }
+    w.l += sum;
+    split8<F16>(p[0], ph[0], pl[0]);
+    split8<F16>(p[1], ph[1], pl[1]);
 }
 
 template <bool F16>
@@ -341,171 +482,561 @@ __device__ __forceinline__ void store4(const Kv4AttnArgs& a, long at, f4v o) {
     }
 }
 
-// Few rows (decode, drafts): a block's waves take the units of its split in
-// turn, 16 rows each.
-template <int HD, bool F16>
-__device__ __forceinline__ void stream_tile(const Kv4AttnArgs& a, const Tile& t, const int* table, int split, float* smem) {
-    constexpr int KS = HD / 32, MT = HD / 16;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int last = min(t.r0 + 15, t.rows - 1);
-    const Units u = units_of(t.pos0 + t.r0 / a.group, t.pos0 + last / a.group, a.window, a.sink);
-    const int u_lo = (int)((long)u.n * split / a.n_split), u_hi = (int)((long)u.n * (split + 1) / a.n_split);
-    const int r = min(t.r0 + i, last);  // rows past the last repeat it
+__device__ __forceinline__ long out_at(const Kv4AttnArgs& a, const Tile& t, int r, int hd) {
+    return (long)(t.q0 + r / a.group) * a.out_stride + (long)(t.head * a.group + r % a.group) * hd;
+}
+
+// A tile whose units several blocks share: blocks [b0, b1].  Each leaves its
+// rows in a slot of its own, two slots a block (the tile that it goes on with
+// and the one that it leaves unfinished; other tiles it does whole).
+struct Shared {
+    int b0, b1;
+    __device__ __forceinline__ bool split() const { return b1 > b0; }
+    __device__ __forceinline__ long slot(int b) const { return b == b0 ? 2L * b + 1 : 2L * b; }
+};
+__device__ __forceinline__ Shared shared_of(const Work& w, const Piece& p) {
+    const int b = blockIdx.x, d = (int)(p.first - (long)b * w.chunk);  // where the tile starts, from this block's start
+    return {d >= 0 ? b : b - (w.chunk - 1 - d) / w.chunk, b + (d + p.n - 1) / w.chunk};
+}
+template <int HD, int R>
+__device__ __forceinline__ unsigned part_at(long slot, int row) {  // floats into the partial rows
+    return (unsigned)((slot * R + row) * (HD + 4));
+}
+
+// Partial rows pass between blocks on different XCDs, whose L2s do not see each
+// other's lines.  They are written and read past the L2s (cache policy sc1, as
+// device-scope atomics are), and the writer waits for its stores before the
+// counter: fences instead would write back and drop the whole L2 once per
+// block (measured: 190 -> 430 us for 64 sequences of up to 16384 tokens at 16
+// splits of their keys).
+constexpr int SC1 = 16;
+struct Parts {
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ void put4(unsigned at, f4v v) const {  // at: floats
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4v, v), rsrc, (int)(at * 4), 0, SC1);
+    }
+    __device__ __forceinline__ f4v get4(unsigned at) const {
+        return __builtin_bit_cast(f4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(at * 4), 0, SC1));
+    }
+};
+__device__ __forceinline__ Parts parts_of(const Kv4AttnArgs& a) {
+    return {__builtin_amdgcn_make_buffer_rsrc(a.part, 0, a.part_bytes, 0x00027000)};
+}
+
+// The shared pieces of a block: the one that it went on with and the one that
+// it leaves unfinished.
+struct Shares {
+    int n = 0;
+    Shared sh[2];
+    Tile t[2];
+    __device__ __forceinline__ void add(const Shared& s, const Tile& tile) {
+        if (n == 0) sh[0] = s, t[0] = tile;
+        else sh[1] = s, t[1] = tile;
+        n++;
+    }
+};
+// A shared tile's rows to one: by the block that finishes last, over the
+// blocks in order.  (The counter is left at 0 for the next call.)
+template <int HD, bool F16, int R, int THREADS>
+__device__ __forceinline__ void join_blocks(const Kv4AttnArgs& a, const Shares& p) {
+    __shared__ int last[2];
+    if (p.n == 0) return;
+    const Parts parts = parts_of(a);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's partial rows have arrived
+    __syncthreads();
+    if (threadIdx.x < (unsigned)p.n) {
+        const Shared& sh = threadIdx.x ? p.sh[1] : p.sh[0];
+        const bool mine = __hip_atomic_fetch_add(a.count + sh.b0, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == sh.b1 - sh.b0;
+        if (mine) __hip_atomic_store(a.count + sh.b0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last[threadIdx.x] = mine;
+    }
+    __syncthreads();
+    constexpr int LPR = HD / 4, RPB = THREADS / LPR, PB = 4;
+    constexpr int RU = R / RPB >= 4 ? 4 : R / RPB >= 2 ? 2 : 1;
+    const int l = threadIdx.x % LPR;
+    for (int k = 0; k < p.n; k++) {
+        if (!last[k]) continue;
+        const Tile& t = k ? p.t[1] : p.t[0];
+        const Shared& sh = k ? p.sh[1] : p.sh[0];
+        // RU rows and PB blocks' parts of them are loaded together: a load past
+        // the L2 takes microseconds, and one after the other they would add up
+        for (int r0 = t.r0 + threadIdx.x / LPR; r0 < t.r1; r0 += RU * RPB) {
+            float m[RU], sum[RU];
+            f4v o[RU];
+#pragma unroll
+            for (int x = 0; x < RU; x++) m[x] = __builtin_inff(), sum[x] = 0.0f, o[x] = f4v{0, 0, 0, 0};
+            for (int b = sh.b0; b <= sh.b1; b += PB) {
+                f4v n[RU][PB], v[RU][PB];
+#pragma unroll
+                for (int x = 0; x < RU; x++)
+#pragma unroll
+                    for (int y = 0; y < PB; y++) {
+                        const unsigned q = part_at<HD, R>(sh.slot(min(b + y, sh.b1)), min(r0 + x * RPB, t.r1 - 1) - t.r0);
+                        n[x][y] = parts.get4(q + HD);
+                        v[x][y] = parts.get4(q + 4 * l);
+                    }
+#pragma unroll
+                for (int x = 0; x < RU; x++)
+#pragma unroll
+                    for (int y = 0; y < PB; y++) {
+                        if (b + y > sh.b1 || n[x][y].x == 0.0f) continue;  // (no key seen)
+                        const float now = fminf(m[x], n[x][y].y);
+                        const float keep = sum[x] != 0.0f ? __builtin_amdgcn_exp2f(now - m[x]) : 0.0f;
+                        const float w = __builtin_amdgcn_exp2f(now - n[x][y].y);
+                        m[x] = now;
+                        sum[x] = sum[x] * keep + w * n[x][y].x;
+                        o[x] = o[x] * keep + v[x][y] * w;
+                    }
+            }
+#pragma unroll
+            for (int x = 0; x < RU; x++) {
+                const int r = r0 + x * RPB;
+                if (r < t.r1) store4<F16>(a, out_at(a, t, r, HD) + 4 * l, o[x] * (sum[x] != 0.0f ? 1.0f / sum[x] : 0.0f));
+            }
+        }
+    }
+}
+
+// A block's W waves hold the same rows over different keys: their sums to
+// one.  acc[m]: O^T tiles, dims 16 m + 4 g + r of row i.  Wave w ends with the
+// tiles m = w, w + W, ... in out.
+constexpr int tiles_of_wave(int hd, int w) { return hd / 16 > w ? hd / 16 / w : 1; }
+template <int HD, int W>
+__device__ __forceinline__ void join_waves(f4v* acc, float nfm, float& l, float* nfm_all, float* smem, f4v* out) {
+    constexpr int MT = HD / 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15;
+    l = rows_sum(l);
+    float* s_n = smem;                 // [W][16]
+    float* s_l = smem + 16 * W;        // [W][16]
+    f4v* s_o = (f4v*)(smem + 32 * W);  // [W][MT tiles][64 lanes], each to its own wave's maximum
+    __syncthreads();                   // the last piece's readers are done
+    if (lane < 16) {
+        s_n[wave * 16 + i] = l != 0.0f ? nfm : __builtin_inff();  // no key seen: no weight (NaN counts as seen)
+        s_l[wave * 16 + i] = l;
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++) s_o[(wave * MT + m) * 64 + lane] = acc[m];
+    __syncthreads();
+    float n = s_n[i];
+#pragma unroll
+    for (int w = 1; w < W; w++) n = fminf(n, s_n[w * 16 + i]);
+    float sum = 0.0f, f[W];
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        const float x = s_l[w * 16 + i];
+        f[w] = x != 0.0f ? __builtin_amdgcn_exp2f(n - s_n[w * 16 + i]) : 0.0f;
+        sum += x * f[w];
+    }
+    l = sum;
+    *nfm_all = n;
+#pragma unroll
+    for (int c = 0; c < tiles_of_wave(HD, W); c++) {
+        const int m = c * W + wave;
+        f4v o = {0, 0, 0, 0};
+        if (m < MT)
+#pragma unroll
+            for (int w = 0; w < W; w++) o += s_o[(w * MT + m) * 64 + lane] * f[w];
+        out[c] = o;
+    }
+}
+
+// Up to 16 rows of a sequence and KV head (decode): a block's waves take the
+// units of its piece in turn.  A wave's K words are free once the scores
+// are done and its V words once the output is: the loads of the unit DEPTH
+// turns later go there and then.  V scales (a lane's operands need all 16 of
+// its tokens', the same for 16 lanes) come as one 64th a lane and pass through
+// LDS, which takes 8 wide loads and 32 registers less than loading them to
+// every lane.
+template <int HD>
+struct Raw {
+    KRow<HD, HD / 32> k[4];
+    u4v v[HD / 32];
+    uint32_t vs[HD / 64];
+    bool v_ok;
+};
+template <int HD, bool F16, int W, int DEPTH>
+__global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
+    constexpr int KS = HD / 32, MT = HD / 16, SROW = HD + 16;
+    __shared__ __align__(16) float smem[32 * W + W * MT * 64 * 4];
+    __shared__ __align__(16) uint8_t s_vs[W][4 * SROW];
+    const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    Work work;
+    Batch batch;
+    if (!work_of<16>(a, work, batch)) return;
+    const int ps = 1 << a.c.ps_shift;
+    Tile t;
+    Units u;
+    Piece part;
+    Raw<HD> raw[DEPTH];
+    int kp[DEPTH], vp[DEPTH];  // pages of the units to load next
+    // (Past the piece's end its last unit is loaded again: behind a branch the
+    // compiler could not tell which loads are in flight and would wait for all.)
+    auto unit_of = [&](int n) { return u.at(max(min(n, part.hi - 1), 0)); };
+    auto pages = [&](int n, int& k, int& v) {
+        k = page_of(a, t.table, k_key(unit_of(n)));
+        v = page_of(a, t.table, v_key(unit_of(n)));
+    };
+    auto load_k = [&](int n, int page, Raw<HD>& w) {
+        bool ok;
+        const int key = k_key(unit_of(n)), off = key & (ps - 1);
+        const uint8_t* p = page_ptr(a, page, key, t.head, ok);
+#pragma unroll
+        for (int x = 0; x < 4; x++) load_krow<HD, KS>(p, ok, ps, off + 4 * x, 0, w.k[x]);
+    };
+    auto load_v = [&](int n, int page, Raw<HD>& w) {
+        const int key = v_key(unit_of(n)), grp = (key & (ps - 1)) >> 4;
+        const uint8_t* p = page_ptr(a, page, key, t.head, w.v_ok);
+        const uint8_t* c = p + ps * (HD / 2) + grp * (HD * 8) + i * 16;
+#pragma unroll
+        for (int b = 0; b < KS; b++) w.v[b] = *gptr<u4v>(c + b * 256);
+        const uint8_t* s = p + ps * HD + ps * (HD / 16) + grp * HD + i * (HD / 16);
+        if constexpr (HD == 64) {
+            w.vs[0] = *gptr<uint32_t>(s);
+        } else if constexpr (HD == 128) {
+            const u2v x = *gptr<u2v>(s);
+            w.vs[0] = x.x, w.vs[1] = x.y;
+        } else {
+            const u4v x = *gptr<u4v>(s);
+            w.vs[0] = x.x, w.vs[1] = x.y, w.vs[2] = x.z, w.vs[3] = x.w;
+        }
+    };
     h8v qh[KS], ql[F16 ? 1 : KS];
     float f;
-    load_q<HD, F16>(a, t, r, qh, ql, f);
-    Row w;
-    row_init(a, t, r, f, w);
-    const int full_hi = (int)(t.pos0 + t.r0 / a.group);  // every row sees keys up to here ..
-    const int full_lo = a.window > 0 ? (int)max(0L, t.pos0 + last / a.group - a.window + 1) : 0;  // .. from here on
-    f4v acc[MT];
+    // the next piece, its q rows and its first units' loads
+    auto begin = [&]() {
+        piece_of<16>(a, work, batch, t, u, part);
+        const int n0 = part.lo + wave;
 #pragma unroll
-    for (int m = 0; m < MT; m++) acc[m] = f4v{0, 0, 0, 0};
-    for (int n = u_lo + wave; n < u_hi; n += 4) {
-        const int unit = u.at(n), key0 = unit * UNIT;
-        KRaw<HD> k;
-        load_k<HD>(a, table, t.head, unit, k);
-        VRaw<HD> v;
-        load_v<HD>(a, table, t.head, unit, t.len, v);
-        f4v c[4];
-        scores<HD, F16>(k, qh, ql, c);
-        float top;
-        const bool whole = key0 + UNIT - 1 <= full_hi && key0 >= full_lo;
-        const bool grow = whole ? row_max<false>(w, key0 + 16 * g, a.sink, c, top) : row_max<true>(w, key0 + 16 * g, a.sink, c, top);
-        if (__any(grow)) {
-            const float nfm = grow ? PBIAS - w.f * top : w.nfm;
-            const float keep = !grow ? 1.0f : w.m == -__builtin_inff() ? 0.0f : exp2f(nfm - w.nfm);
-            if (grow) w.m = top;
-            w.nfm = nfm;
-            w.l *= keep;
+        for (int d = 0; d < DEPTH; d++) pages(n0 + W * d, kp[d], vp[d]);
+        load_q<HD, F16>(a, t, min(t.r0 + i, t.r1 - 1), qh, ql, f);  // rows past the last repeat it
 #pragma unroll
-            for (int m = 0; m < MT; m++) acc[m] *= keep;
+        for (int d = 0; d < DEPTH; d++) {
+            load_k(n0 + W * d, kp[d], raw[d]);
+            load_v(n0 + W * d, vp[d], raw[d]);
         }
-        float p[2][8];
+        pages(n0 + W * DEPTH, kp[0], vp[0]);
+    };
+    Shares shares;
+    begin();
+    for (;;) {
+        Row w;
+        row_init(a, t, min(t.r0 + i, t.r1 - 1), f, w);
+        const Whole whole = whole_of(a, t, t.r0, t.r1);
+        f4v acc[MT];
 #pragma unroll
-        for (int x = 0; x < 4; x++)
+        for (int m = 0; m < MT; m++) acc[m] = f4v{0, 0, 0, 0};
+        for (int base = part.lo + wave; base < part.hi; base += W * DEPTH) {
 #pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y], w.f, w.nfm));
-                p[x >> 1][(x & 1) * 4 + y] = e;
-                w.l += e;
+            for (int d = 0; d < DEPTH; d++) {
+                const int n = base + W * d;
+                if (n >= part.hi) break;
+                Raw<HD>& x = raw[d];
+                const int key0 = u.at(n) * UNIT, next = n + W * DEPTH;
+                f4v c[4];
+#pragma unroll
+                for (int y = 0; y < 4; y++) c[y] = f4v{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const h8v o = k_operand(x.k[y].w[s], x.k[y].scale(s));
+                        c[y] = mfma(o, qh[s], c[y]);
+                        if constexpr (!F16) c[y] = mfma(o, ql[s], c[y]);
+                    }
+                const int vnext = vp[0];
+                load_k(next, kp[0], x);
+                pages(next + W, kp[0], vp[0]);
+                h8v ph[2], pl[2];
+                softmax<F16, MT>(w, whole.has(key0), key0, a.sink, c, acc, ph, pl);
+                // scales of this lane: tokens 16 g + HD / 32 * (i % (512 / HD)) .. of block i / (512 / HD)
+                uint32_t vs[HD / 64];
+#pragma unroll
+                for (int y = 0; y < HD / 64; y++) vs[y] = x.vs[y];
+                if (key0 + UNIT > t.len || !x.v_ok) {
+                    const int key = key0 + 16 * g + (HD / 32) * (i % (512 / HD)), len = x.v_ok ? t.len : 0;
+#pragma unroll
+                    for (int y = 0; y < HD / 64; y++)
+                        vs[y] = key + 2 * y + 1 < len ? vs[y] : key + 2 * y < len ? vs[y] & 0xFFFFu : 0;
+                }
+                uint8_t* sv = s_vs[wave];
+                if constexpr (HD == 64) *(uint32_t*)(sv + g * SROW + i * 4) = vs[0];
+                else if constexpr (HD == 128) *(u2v*)(sv + g * SROW + i * 8) = u2v{vs[0], vs[1]};
+                else *(u4v*)(sv + g * SROW + i * 16) = u4v{vs[0], vs[1], vs[2], vs[3]};
+#pragma unroll
+                for (int b = 0; b < KS; b++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        VPart v;
+                        v.w = y ? u2v{x.v[b].z, x.v[b].w} : u2v{x.v[b].x, x.v[b].y};
+                        v.s = *(const u4v*)(sv + g * SROW + b * 32 + y * 16);
+                        h8v lo, hi;
+                        v_operands(v, lo, hi);
+                        acc[2 * b] = mfma(lo, ph[y], acc[2 * b]);
+                        acc[2 * b + 1] = mfma(hi, ph[y], acc[2 * b + 1]);
+                        if constexpr (!F16) {
+                            acc[2 * b] = mfma(lo, pl[y], acc[2 * b]);
+                            acc[2 * b + 1] = mfma(hi, pl[y], acc[2 * b + 1]);
+                        }
+                    }
+                load_v(next, vnext, x);
             }
-        h8v ph[2], pl[2];
-        split8<F16>(p[0], ph[0], pl[0]);
-        split8<F16>(p[1], ph[1], pl[1]);
+        }
+        // the next piece's loads are on their way while this one is put together
+        const Tile done = t;
+        const Shared sh = shared_of(work, part);
+        const bool more = work.left > 0;
+        if (more) begin();
+        float l = w.l, nfm;
+        f4v o[tiles_of_wave(HD, W)];
+        join_waves<HD, W>(acc, w.nfm, l, &nfm, smem, o);
+        if (done.r0 + i < done.r1 && wave < MT) {
+            if (!sh.split()) {
+                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+                const long at = out_at(a, done, done.r0 + i, HD);
 #pragma unroll
-        for (int b = 0; b < HD / 32; b++)
+                for (int c = 0; c < tiles_of_wave(HD, W); c++) store4<F16>(a, at + 16 * (c * W + wave) + 4 * g, o[c] * inv);
+            } else {
+                const Parts parts = parts_of(a);
+                const unsigned row = part_at<HD, 16>(sh.slot(blockIdx.x), i);
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
+                for (int c = 0; c < tiles_of_wave(HD, W); c++) parts.put4(row + 16 * (c * W + wave) + 4 * g, o[c]);
+                if (wave == 0 && g == 0) parts.put4(row + HD, f4v{l, nfm, 0, 0});
+            }
+        }
+        if (sh.split()) shares.add(sh, done);
+        if (!more) break;
+    }
+    join_blocks<HD, F16, 16, 64 * W>(a, shares);
+}
+
+// More rows (drafts, prompts): W waves with 16 NT rows each, over the same
+// units.  Each wave turns its share of a unit's codes into f16 operands in
+// LDS, in the order in which a lane reads them (16 bytes a lane, no bank
+// conflict), one unit ahead of their use where two buffers fit; the next
+// unit's codes are in flight meanwhile (the barrier orders LDS only).
+template <int HD, bool F16, int W, int NT>
+__global__ __launch_bounds__(64 * W, HD == 256 && NT == 2 ? 1 : 2) void k_kv4_attn_chunk(Kv4AttnArgs a) {
+    constexpr int KS = HD / 32, MT = HD / 16, R = 16 * NT * W;
+    constexpr int KW = 4 * KS / W;                   // K words a lane stages
+    constexpr int NJ = 2 * KS >= W ? 2 * KS / W : 1;  // V parts a lane stages (HD 64, 8 waves: the first 4)
+    constexpr int BUFS = HD == 256 ? 1 : 2;
+    __shared__ __align__(16) h8v s_k[BUFS][4 * KS * 64];  // [word][key tile][lane]
+    __shared__ __align__(16) h8v s_v[BUFS][4 * KS * 64];  // [block][part][low, high][lane]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    Work work;
+    Batch batch;
+    Tile t;
+    if (a.whole) {
+        if (!whole_tile<R>(a, t)) return;
+        work.left = 0;
+    } else if (!work_of<R>(a, work, batch)) {
+        return;
+    }
+    const int ps = 1 << a.c.ps_shift;
+    Shares shares;
+  do {
+    Units u;
+    Piece part;
+    if (a.whole) {
+        u = tile_units(a, t, t.r0, t.r1);
+        part.lo = 0;
+        part.hi = u.n;
+    } else {
+        piece_of<R>(a, work, batch, t, u, part);
+    }
+    __syncthreads();  // the last piece's operands are read
+    const int head = t.head;
+    const int kt = wave & 3, s0 = W == 8 ? (wave >> 2) * KW : 0, j0 = wave * NJ;
+    const bool stage_v = j0 < 2 * KS;
+    KRow<HD, KW> k;
+    VPart v[NJ];
+    int kp = 0, vp = 0;
+    auto unit_of = [&](int n) { return u.at(max(min(n, part.hi - 1), 0)); };  // (as above: no branch around loads)
+    auto pages = [&](int n) {
+        kp = page_of(a, t.table, k_key(unit_of(n)));
+        vp = page_of(a, t.table, v_key(unit_of(n)));
+    };
+    bool v_ok = true;
+    auto load = [&](int n) {
+        bool ok;
+        const int unit = unit_of(n);
+        const uint8_t* p = page_ptr(a, kp, k_key(unit), head, ok);
+        load_krow<HD, KW>(p, ok, ps, (k_key(unit) & (ps - 1)) + 4 * kt, s0, k);
+        if (stage_v) {
+            p = page_ptr(a, vp, v_key(unit), head, v_ok);
+#pragma unroll
+            for (int j = 0; j < NJ; j++) load_vpart<HD>(p, ps, v_key(unit) & (ps - 1), (j0 + j) >> 1, (j0 + j) & 1, v[j]);
+        }
+    };
+    pages(part.lo);
+    // this wave's rows; a wave without any repeats the tile's last and stores nothing
+    const int r0 = min(t.r0 + wave * 16 * NT, t.r1 - 1), r1 = min(t.r0 + (wave + 1) * 16 * NT, t.r1);
+    h8v qh[NT][KS], ql[NT][F16 ? 1 : KS];
+    Row w[NT];
+    f4v acc[NT][MT];
+#pragma unroll
+    for (int x = 0; x < NT; x++) {
+        const int r = min(r0 + 16 * x + i, t.r1 - 1);
+        float f;
+        load_q<HD, F16>(a, t, r, qh[x], ql[x], f);
+        row_init(a, t, r, f, w[x]);
+#pragma unroll
+        for (int m = 0; m < MT; m++) acc[x][m] = f4v{0, 0, 0, 0};
+    }
+    load(part.lo);
+    pages(part.lo + 1);
+    const Whole whole = whole_of(a, t, r0, max(r1, r0 + 1));
+    const int first_lo = a.window > 0 ? (int)max(0L, t.pos0 + r0 / a.group - a.window + 1) : 0;
+    const int last_hi = (int)(t.pos0 + (max(r1, r0 + 1) - 1) / a.group);
+    for (int n = part.lo; n < part.hi; n++) {
+        const int key0 = u.at(n) * UNIT;
+        h8v* bk = s_k[BUFS == 2 ? (n - part.lo) & 1 : 0];
+        h8v* bv = s_v[BUFS == 2 ? (n - part.lo) & 1 : 0];
+        if constexpr (BUFS == 1) lds_barrier();  // the last unit's readers are done
+#pragma unroll
+        for (int s = 0; s < KW; s++) bk[((s0 + s) * 4 + kt) * 64 + lane] = k_operand(k.w[s], k.scale(s));
+        if (stage_v) {
+            if (key0 + UNIT > t.len || !v_ok) {
+#pragma unroll
+                for (int j = 0; j < NJ; j++) cut_vpart(v[j], key0 + 16 * g + 8 * ((j0 + j) & 1), v_ok ? t.len : 0);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
                 h8v lo, hi;
-                const uint32_t sc[4] = {v.s[b][s].x, v.s[b][s].y, v.s[b][s].z, v.s[b][s].w};
-                v_operands(s ? v.w[b].z : v.w[b].x, s ? v.w[b].w : v.w[b].y, sc, lo, hi);
-                acc[2 * b] = mfma(lo, ph[s], acc[2 * b]);
-                acc[2 * b + 1] = mfma(hi, ph[s], acc[2 * b + 1]);
+                v_operands(v[j], lo, hi);
+                bv[((j0 + j) * 2 + 0) * 64 + lane] = lo;
+                bv[((j0 + j) * 2 + 1) * 64 + lane] = hi;
+            }
+        }
+        load(n + 1);
+        pages(n + 2);
+        lds_barrier();
+        // nothing here for this wave's rows: no query of it sees a key of the unit
+        if (r1 <= r0 || key0 > last_hi || (key0 + UNIT <= first_lo && key0 >= a.sink)) continue;
+        f4v c[NT][4];
+#pragma unroll
+        for (int x = 0; x < NT; x++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) c[x][y] = f4v{0, 0, 0, 0};
+        // Operands are read one step ahead of their products (the fences keep
+        // them there: read where they are used, every pair waits out the LDS).
+        h8v cur[4], nxt[4];
+#pragma unroll
+        for (int y = 0; y < 4; y++) cur[y] = bk[y * 64 + lane];
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+#pragma unroll
+            for (int y = 0; y < 4; y++) nxt[y] = s + 1 < KS ? bk[((s + 1) * 4 + y) * 64 + lane] : bv[y * 64 + lane];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < 4; y++)
+#pragma unroll
+                for (int x = 0; x < NT; x++) c[x][y] = mfma(cur[y], qh[x][s], c[x][y]);
+            if constexpr (!F16) {
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+#pragma unroll
+                    for (int x = 0; x < NT; x++) c[x][y] = mfma(cur[y], ql[x][s], c[x][y]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < 4; y++) cur[y] = nxt[y];
+        }
+        h8v ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int x = 0; x < NT; x++) softmax<F16, MT>(w[x], whole.has(key0), key0, a.sink, c[x], acc[x], ph[x], pl[x]);
+#pragma unroll
+        for (int b = 0; b < KS; b++) {  // cur: tokens 0-7 low, high nibbles' dims, tokens 8-15
+            if (b + 1 < KS) {
+#pragma unroll
+                for (int y = 0; y < 4; y++) nxt[y] = bv[((b + 1) * 4 + y) * 64 + lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+#pragma unroll
+                for (int x = 0; x < NT; x++) {
+                    acc[x][2 * b] = mfma(cur[2 * y], ph[x][y], acc[x][2 * b]);
+                    acc[x][2 * b + 1] = mfma(cur[2 * y + 1], ph[x][y], acc[x][2 * b + 1]);
+                }
                 if constexpr (!F16) {
-                    acc[2 * b] = mfma(lo, pl[s], acc[2 * b]);
-                    acc[2 * b + 1] = mfma(hi, pl[s], acc[2 * b + 1]);
+#pragma unroll
+                    for (int x = 0; x < NT; x++) {
+                        acc[x][2 * b] = mfma(cur[2 * y], pl[x][y], acc[x][2 * b]);
+                        acc[x][2 * b + 1] = mfma(cur[2 * y + 1], pl[x][y], acc[x][2 * b + 1]);
+                    }
                 }
             }
-    }
-    float l = w.l, nfm;
-    f4v o[HD / 64];
-    join_waves<HD>(acc, w.nfm, l, &nfm, smem, o);
-    if (t.r0 + i > last) return;
-    const int tok = t.q0 + r / a.group, h = t.head * a.group + r % a.group;
-    if (a.n_split == 1) {
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        const long at = (long)tok * a.out_stride + (long)h * HD;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < HD / 64; c++) store4<F16>(a, at + 16 * (4 * c + wave) + 4 * g, o[c] * inv);
+            for (int y = 0; y < 4; y++) cur[y] = nxt[y];
+        }
+    }
+    const Shared sh = a.whole ? Shared{0, 0} : shared_of(work, part);
+#pragma unroll
+    for (int x = 0; x < NT; x++) {
+        const float l = rows_sum(w[x].l);
+        const int r = r0 + 16 * x + i;
+        if (r >= r1) continue;
+        if (!sh.split()) {
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+            const long at = out_at(a, t, r, HD);
+#pragma unroll
+            for (int m = 0; m < MT; m++) store4<F16>(a, at + 16 * m + 4 * g, acc[x][m] * inv);
+        } else {
+            const Parts parts = parts_of(a);
+            const unsigned row = part_at<HD, R>(sh.slot(blockIdx.x), r - t.r0);
+#pragma unroll
+            for (int m = 0; m < MT; m++) parts.put4(row + 16 * m + 4 * g, acc[x][m]);
+            if (g == 0) parts.put4(row + HD, f4v{l, w[x].nfm, 0, 0});
+        }
+    }
+    if (sh.split()) shares.add(sh, t);
+  } while (work.left > 0);
+    join_blocks<HD, F16, R, 64 * W>(a, shares);
+}
+
+template <int HD, bool F16>
+void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)p.grid);
+    if (p.rows == 16) {
+        hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, HD == 256 ? 2 : 1>), grid, dim3(256), 0, st, a);
+    } else if (p.rows == 64) {
+        hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 4, 1>), grid, dim3(256), 0, st, a);
     } else {
-        float* row = a.part + (((long)tok * a.n_head + h) * a.n_split + split) * (HD + 4);
-#pragma unroll
-        for (int c = 0; c < HD / 64; c++) *(f4v*)(row + 16 * (4 * c + wave) + 4 * g) = o[c];
-        if (wave == 0 && g == 0) *(f4v*)(row + HD) = f4v{l, nfm, 0, 0};
+        if constexpr (HD == 256 && F16) hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 4, 2>), grid, dim3(256), 0, st, a);
+        else if constexpr (HD != 256) hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 8, 2>), grid, dim3(512), 0, st, a);
     }
-}
-
-template <int HD, bool F16>
-__global__ __launch_bounds__(256) void k_kv4_attn(Kv4AttnArgs a) {
-    __shared__ __align__(16) float smem[128 + 4 * 4 * 64 * 4];
-    unsigned id = blockIdx.x;
-    const int split = id % a.n_split;
-    id /= a.n_split;
-    const int head = id % a.c.n_kv;
-    id /= a.c.n_kv;
-    const int tile = id % a.tiles, seq = id / a.tiles;
-    Tile t;
-    seq_of(a, seq, head, t);
-    const int* table = a.block_table + (long)seq * a.max_blocks;
-    // (more tiles than the caller's max_q said: the blocks go round again)
-    for (t.r0 = tile * 16; t.r0 < t.rows; t.r0 += a.tiles * 16) stream_tile<HD, F16>(a, t, table, split, smem);
-}
-
-// Splits of a row to one.  A row's lanes: HD / 4, four dims each.
-template <int HD, bool F16>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
-    constexpr int LPR = HD / 4, RPB = 256 / LPR;
-    const long row = (long)blockIdx.x * RPB + threadIdx.x / LPR;
-    if (row >= (long)a.n_tok * a.n_head) return;
-    const int tok = (int)(row / a.n_head), h = (int)(row - (long)tok * a.n_head);
-    if (tok < a.cu_q[0] || tok >= a.cu_q[a.n_seq]) return;  // rows of no sequence stay as they are
-    const int l = threadIdx.x % LPR;
-    const float* p = a.part + row * a.n_split * (HD + 4);
-    float n = __builtin_inff();
-    for (int s = 0; s < a.n_split; s++)
-        if (p[s * (HD + 4) + HD] != 0.0f) n = fminf(n, p[s * (HD + 4) + HD + 1]);
-    float sum = 0.0f;
-    f4v o = {0, 0, 0, 0};
-    for (int s = 0; s < a.n_split; s++) {
-        const float* q = p + s * (HD + 4);
-        if (q[HD] == 0.0f) continue;
-        const float w = exp2f(n - q[HD + 1]);
-        sum += w * q[HD];
-        o += *(const f4v*)(q + 4 * l) * w;
-    }
-    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-    store4<F16>(a, (long)tok * a.out_stride + (long)h * HD + 4 * l, o * inv);
-}
-
-template <int HD, bool F16>
-int attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
-    const long grid = (long)a.n_seq * p.tiles * a.c.n_kv * p.n_split;
-    if (grid > 0x7FFFFFFFL) return -1;
-    hipLaunchKernelGGL((k_kv4_attn<HD, F16>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    if (p.n_split > 1) {
-        constexpr int RPB = 256 / (HD / 4);
-        const long rows = (long)a.n_tok * a.n_head;
-        hipLaunchKernelGGL((k_kv4_join<HD, F16>), dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), 0, st, a);
-    }
-    return 0;
 }
 
 }  // namespace
 
-Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, long max_len,
-                          int window, int sink, int cus) {
+Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, int cus) {
     Kv4AttnPlan p = {};
-    (void)f16;
-    const int group = n_head / n_kv;
-    p.rows = 16;
-    p.tiles = (int)(((long)max_q * group + p.rows - 1) / p.rows);
-    long keys = max_len;
-    if (window > 0) keys = min(keys, (long)window + max_q + sink);
-    const long units = max(1L, (keys + UNIT - 1) / UNIT), base = (long)n_seq * p.tiles * n_kv;
-    const long want = 3L * cus;
-    p.n_split = (int)max(1L, min(min((want + base - 1) / base, (units + 3) / 4), 128L));
-    p.work = p.n_split > 1 ? (size_t)n_tok * n_head * p.n_split * (hd + 4) * sizeof(float) : 0;
+    const int group = n_head / n_kv, big = hd != 256 ? 256 : f16 ? 128 : 64;
+    const long rows = (long)max_q * group;
+    auto tiles = [&](int r) { return ((long)n_tok * group / r + n_seq) * n_kv; };
+    p.rows = rows <= 16 ? 16 : 64;
+    if (rows > 64 && (long)n_tok * group / big * n_kv >= cus / 2) p.rows = big;
+    p.whole = rows > 16 && (long)n_tok * group / p.rows * n_kv >= cus / 2;
+    p.grid = p.whole ? tiles(p.rows) : (p.rows == 16 && hd != 256 ? 2 : 1) * cus;
+    p.chunk = p.rows == 16 ? 4 : 2;
+    p.part_bytes = p.whole ? 0 : (size_t)p.grid * 2 * p.rows * (hd + 4) * sizeof(float);
+    p.work = p.whole ? 0 : KV4_COUNT_BYTES + p.part_bytes;
     return p;
 }
 
-int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, hipStream_t st) {
-    a.tiles = p.tiles;
-    a.n_split = p.n_split;
+int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, void* work, hipStream_t st) {
+    if (p.grid > 0x7FFFFFFFL) return -1;
+    a.whole = p.whole;
+    a.part_bytes = (unsigned)p.part_bytes;
+    a.chunk = p.chunk;
+    a.count = (int*)work;
+    a.part = (float*)((char*)work + KV4_COUNT_BYTES);
     switch (a.c.hd) {
-    case 64: return f16 ? attn_run<64, true>(a, p, st) : attn_run<64, false>(a, p, st);
-    case 128: return f16 ? attn_run<128, true>(a, p, st) : attn_run<128, false>(a, p, st);
-    case 256: return f16 ? attn_run<256, true>(a, p, st) : attn_run<256, false>(a, p, st);
+    case 64: f16 ? attn_run<64, true>(a, p, st) : attn_run<64, false>(a, p, st); return 0;
+    case 128: f16 ? attn_run<128, true>(a, p, st) : attn_run<128, false>(a, p, st); return 0;
+    case 256: f16 ? attn_run<256, true>(a, p, st) : attn_run<256, false>(a, p, st); return 0;
     }
     return -1;
 }

@@ -605,8 +605,9 @@ int draco_kv4_read(const DracoKv4* cache, const int* slot, int n, float* k, floa
  * smaller values only cost speed.  A length past max_blocks pages, or a page
  * outside the pool that a row sees, gives NaN.  work / work_bytes: at least
  * draco_kv4_attn_workspace(cache, p) bytes (it reads sizes only), 16-byte
- * aligned, any content; calls that overlap need their own.  Results do not
- * depend on the other rows of the batch's values, and a call's are the same
+ * aligned.  Its first 16 KiB (counters) are 0 before its first use; calls of
+ * any shapes leave them 0 again, so one allocation of the largest size serves
+ * them all.  Calls that overlap need their own.  A call's results are the same
  * every time. */
 typedef struct {
     int code;

@@ -25,6 +25,13 @@ def dev():
     h.free()
 
 
+def _workspace(n):
+    """Counters 0, the rest anything."""
+    w = np.full(n, 0xFF, np.uint8)
+    w[:16384] = 0
+    return w
+
+
 class Cache:
     """A pool of pages, all bytes 0xFF at first (NaN scales), and block tables over shuffled pages."""
 
@@ -88,7 +95,7 @@ class Cache:
                              block_table=d.up(self.table))
         need = self.L.draco_kv4_attn_workspace(ct.byref(self.desc), ct.byref(a))
         if need:
-            a.work, a.work_bytes = d.up(np.full(need, 0xFF, np.uint8)), need
+            a.work, a.work_bytes = d.up(_workspace(need)), need
         return a
 
     def attn(self, q, cu, lens, code=F32, stream=None, **kw):
@@ -96,6 +103,8 @@ class Cache:
         out = self.dev.up(fill)
         a = self.attn_args(q, out, cu, lens, code=code, **kw)
         self.lib.check(self.L.draco_kv4_attn(ct.byref(self.desc), ct.byref(a), stream), "draco_kv4_attn")
+        if a.work:
+            assert not self.dev.down(a.work, 4096, np.int32).any()  # counters left at 0
         return self.dev.down(out, q.shape, NP[code])
 
 
@@ -519,7 +528,7 @@ def _session(dev, hd=128, nh=8, nkv=2, ps=16, n_seq=5, steps=6):
                       max_blocks=c.width, q=s["qo"], out=s["out"], q_stride=nh * hd, out_stride=nh * hd, cu_q=s["cu"], kv_len=s["kv"],
                       block_table=s["bt"])
     need = c.L.draco_kv4_attn_workspace(ct.byref(c.desc), ct.byref(att))
-    att.work, att.work_bytes = dev.up(np.full(max(need, 16), 0xFF, np.uint8)), need
+    att.work, att.work_bytes = dev.up(_workspace(max(need, 16))), need
 
     def call(stream):
         for f, a in ((c.L.draco_kv_plan, (ct.byref(plan),)), (c.L.draco_kv4_append, (ct.byref(c.desc), ct.byref(app))),
