@@ -3,8 +3,8 @@
 //
 // need_s = ceil((len_s + q_s) / ps) - ceil(len_s / ps) pages; with first_s the
 // exclusive prefix sum of need, the k-th page taken is free_list[n_free - 1 -
-// k].  Every block computes the prefix sums of all sequences itself, 1024 at a
-// time (one sequence per thread; a few KB that all blocks read from L2), and
+// k].  Every block computes the prefix sums of all sequences itself, a tile at
+// a time (one sequence per thread; a few KB that all blocks read from L2), and
 // then serves its own part of the tokens and of the block tables, so one
 // launch does without a device-wide wait.  What the call may write over its
 // own inputs (kv_len_out, n_free_out) is written by the block that finishes
@@ -14,57 +14,48 @@
 
 #include "dev_common.h"
 #include "kv4.h"
+#include "wave_scan.h"
 
 namespace draco {
 namespace {
 
-constexpr int TILE = 1024;  // sequences per pass, threads per block
-
-// Inclusive sums of (a, b) over the block's threads (64 bits: lengths come
-// unchecked from device memory).  red: 2 * 16 values of LDS.
+// Inclusive sums of (a, b) over the block's THREADS threads and their totals
+// (64 bits: lengths come unchecked from device memory).  red: 2 * 16 longs of
+// LDS; every wave adds up the waves before it in its own lanes.
 struct Sum2 {
     long a, b;
 };
-__device__ __forceinline__ Sum2 block_scan(Sum2 v, long* red) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (int d = 1; d < 64; d <<= 1) {
-        const long a = __shfl_up(v.a, d), b = __shfl_up(v.b, d);
-        if (lane >= d) {
-            v.a += a;
-            v.b += b;
-        }
+template <int THREADS>
+__device__ __forceinline__ Sum2 block_scan(Sum2 v, Sum2& total, long* red) {
+    constexpr int W = THREADS / 64;
+    const int lane = threadIdx.x & 63, w = uni((int)threadIdx.x >> 6);
+    v = {wave_scan(v.a), wave_scan(v.b)};
+    if constexpr (W == 1) {
+        total = {lane_of(v.a, 63), lane_of(v.b, 63)};
+        return v;
     }
     __syncthreads();
     if (lane == 63) {
-        red[2 * w] = v.a;
-        red[2 * w + 1] = v.b;
+        red[w] = v.a;
+        red[16 + w] = v.b;
     }
     __syncthreads();
-    for (int i = 0; i < w; i++) {
-        v.a += red[2 * i];
-        v.b += red[2 * i + 1];
-    }
+    const long a = wave_scan(lane < W ? red[lane] : 0L), b = wave_scan(lane < W ? red[16 + lane] : 0L);
+    total = {lane_of(a, W - 1), lane_of(b, W - 1)};
+    if (w) v = {v.a + lane_of(a, w - 1), v.b + lane_of(b, w - 1)};
     return v;
-}
-__device__ __forceinline__ Sum2 block_total(const long* red) {
-    Sum2 t = {0, 0};
-    for (int i = 0; i < TILE / 64; i++) {
-        t.a += red[2 * i];
-        t.b += red[2 * i + 1];
-    }
-    return t;
 }
 
 __device__ __forceinline__ int pages_of(long len, int sh) { return (int)((len + (1 << sh) - 1) >> sh); }
 
 // The last block to arrive (its counter left at 0 again); others return false.
+// Only reads lie before it, and a block's are done when it arrives.
 __device__ __forceinline__ bool last_block(int* ticket, int* flag) {
     __syncthreads();
     if (threadIdx.x == 0) {
-        __threadfence();
-        const int n = atomicAdd(ticket, 1);
+        const int n = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *flag = n == (int)gridDim.x - 1;
-        if (*flag) *ticket = 0;
+        if (*flag) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     return *flag != 0;
@@ -77,6 +68,7 @@ struct Seq {  // one sequence of a tile
 };
 
 // Sequence base + threadIdx.x; row / page: the sums of the tiles before.
+template <int TILE>
 __device__ __forceinline__ Seq plan_seq(const KvPlanArgs& a, int base, long& row, long& page, int n_free, long* red) {
     Seq s = {};
     const int i = base + (int)threadIdx.x;
@@ -89,12 +81,12 @@ __device__ __forceinline__ Seq plan_seq(const KvPlanArgs& a, int base, long& row
         fits = (long)s.old + s.q <= cap;
         s.need = fits ? pages_of((long)s.old + s.q, a.ps_shift) - s.have : 0;
     }
-    const Sum2 in = block_scan({s.q, s.need}, red);
+    Sum2 all;
+    const Sum2 in = block_scan<TILE>({s.q, s.need}, all, red);
     s.cu = row + in.a - s.q;
     s.first = page + in.b - s.need;
-    const Sum2 t = block_total(red);
-    row += t.a;
-    page += t.b;
+    row += all.a;
+    page += all.b;
     s.ok = fits && s.cu + s.q <= a.n_tok && (s.need == 0 || s.first + s.need <= n_free);
     return s;
 }
@@ -104,17 +96,19 @@ __device__ __forceinline__ int taken_page(const KvPlanArgs& a, int n_free, long 
     return (unsigned)p < (unsigned)a.n_pages ? p : -1;
 }
 
+template <int TILE>
 __global__ __launch_bounds__(TILE) void k_kv_plan(KvPlanArgs a) {
-    __shared__ long red[2 * TILE / 64];
+    __shared__ long red[32];
     __shared__ int s_cu[TILE + 1], s_old[TILE], s_first[TILE], s_have[TILE], s_need[TILE];
     __shared__ int flag;
     const int tid = threadIdx.x;
     const int n_free = min(max(*a.n_free, 0), a.n_pages);
     const int per = (a.n_tok + (int)gridDim.x - 1) / (int)gridDim.x;  // this block's tokens
-    const int t0 = min(a.n_tok, per * (int)blockIdx.x), t1 = min(a.n_tok, t0 + per);
+    const int t0 = min((long)a.n_tok, (long)per * blockIdx.x), t1 = min(a.n_tok, t0 + per);
     long row = 0, page = 0;
+    Seq s = {};
     for (int base = 0; base < a.n_seq; base += TILE) {
-        const Seq s = plan_seq(a, base, row, page, n_free, red);
+        s = plan_seq<TILE>(a, base, row, page, n_free, red);
         const int n = min(TILE, a.n_seq - base);
         s_cu[tid] = (int)min(s.cu, (long)a.n_tok);
         if (tid == n - 1) s_cu[n] = (int)min(s.cu + s.q, (long)a.n_tok);
@@ -127,10 +121,6 @@ __global__ __launch_bounds__(TILE) void k_kv_plan(KvPlanArgs a) {
             if (base == 0 && tid == 0) a.cu_q[0] = 0;
             a.cu_q[base + tid + 1] = s_cu[tid + 1];
         }
-        // block tables: a wave per sequence, its new pages over the lanes
-        for (int i = (int)blockIdx.x * (TILE / 64) + (tid >> 6); i < n; i += (int)gridDim.x * (TILE / 64))
-            for (int b = tid & 63; b < s_need[i]; b += 64)
-                a.block_table[(long)(base + i) * a.max_blocks + s_have[i] + b] = taken_page(a, n_free, (long)s_first[i] + b);
         // this block's tokens that belong to the tile
         for (int t = max(t0, s_cu[0]) + tid; t < min(t1, s_cu[n]); t += TILE) {
             int lo = 0, hi = n;  // the last i with s_cu[i] <= t
@@ -150,7 +140,11 @@ __global__ __launch_bounds__(TILE) void k_kv_plan(KvPlanArgs a) {
             a.slot[t] = slot;
             if (a.pos) a.pos[t] = pos;
         }
-        __syncthreads();
+        // block tables: a wave per sequence, its new pages over the lanes
+        for (int i = (int)blockIdx.x * (TILE / 64) + (tid >> 6); i < n; i += (int)gridDim.x * (TILE / 64))
+            for (int b = tid & 63; b < s_need[i]; b += 64)
+                a.block_table[(long)(base + i) * a.max_blocks + s_have[i] + b] = taken_page(a, n_free, (long)s_first[i] + b);
+        if (base + TILE < a.n_seq) __syncthreads();
     }
     // rows behind the last sequence: no slot
     for (int t = (int)max((long)t0, min(row, (long)a.n_tok)) + tid; t < t1; t += TILE) {
@@ -160,24 +154,22 @@ __global__ __launch_bounds__(TILE) void k_kv_plan(KvPlanArgs a) {
     if (a.n_seq == 0 && blockIdx.x == 0 && tid == 0) a.cu_q[0] = 0;
     // lengths and the list's count, behind every block's reads of them
     if (gridDim.x > 1 && !last_block(a.ticket, &flag)) return;
-    row = page = 0;
+    const long rows = row;
     long took = 0, refused = 0;
+    row = page = 0;
     for (int base = 0; base < a.n_seq; base += TILE) {
-        const Seq s = plan_seq(a, base, row, page, n_free, red);
+        if (a.n_seq > TILE) s = plan_seq<TILE>(a, base, row, page, n_free, red);  // (else the tile's are still here)
         const bool real = base + tid < a.n_seq;
-        __syncthreads();
-        const Sum2 in = block_scan({s.ok ? s.need : 0, real && !s.ok}, red);
-        (void)in;
-        const Sum2 t = block_total(red);
-        took += t.a;
-        refused += t.b;
+        Sum2 all;
+        block_scan<TILE>({s.ok ? s.need : 0, real && !s.ok}, all, red);
+        took += all.a;
+        refused += all.b;
         if (real) a.kv_len_out[base + tid] = s.ok ? s.old + s.q : a.kv_len[base + tid];
-        __syncthreads();
     }
     if (tid == 0) {
         *a.n_free_out = n_free - (int)took;
         a.status[0] = (int)refused;
-        a.status[1] = (int)min(max(row - a.n_tok, 0L), (long)INT_MAX);
+        a.status[1] = (int)min(max(rows - a.n_tok, 0L), (long)INT_MAX);
     }
 }
 
@@ -185,6 +177,7 @@ struct Rel {
     int len, keep, have, want;
     long first;
 };
+template <int TILE>
 __device__ __forceinline__ Rel release_seq(const KvReleaseArgs& a, int base, long& page, long* red) {
     Rel s = {};
     const int i = base + (int)threadIdx.x;
@@ -195,29 +188,29 @@ __device__ __forceinline__ Rel release_seq(const KvReleaseArgs& a, int base, lon
         s.have = pages_of(s.len, a.ps_shift);
         s.want = pages_of(s.keep, a.ps_shift);
     }
-    const Sum2 in = block_scan({s.have - s.want, 0}, red);
+    Sum2 all;
+    const Sum2 in = block_scan<TILE>({s.have - s.want, 0}, all, red);
     s.first = page + in.a - (s.have - s.want);
-    page += block_total(red).a;
+    page += all.a;
     return s;
 }
 
 // The released pages' ordinals run over sequences and blocks as a plan's do;
 // page k of n goes to free_list[n_free + n - 1 - k], so that a release of what
 // a plan took restores the list.
+template <int TILE>
 __global__ __launch_bounds__(TILE) void k_kv_release(KvReleaseArgs a) {
-    __shared__ long red[2 * TILE / 64];
+    __shared__ long red[32];
     __shared__ int s_want[TILE], s_go[TILE];
     __shared__ long s_first[TILE];
     __shared__ int flag;
     const int tid = threadIdx.x;
     const long n_free = min(max(*a.n_free, 0), a.n_pages);
     long all = 0, page = 0;
+    Rel s = {};
+    for (int base = 0; base < a.n_seq; base += TILE) s = release_seq<TILE>(a, base, all, red);
     for (int base = 0; base < a.n_seq; base += TILE) {
-        release_seq(a, base, all, red);
-        __syncthreads();
-    }
-    for (int base = 0; base < a.n_seq; base += TILE) {
-        const Rel s = release_seq(a, base, page, red);
+        if (a.n_seq > TILE) s = release_seq<TILE>(a, base, page, red);  // (else the tile's are still here)
         const int n = min(TILE, a.n_seq - base);
         s_want[tid] = s.want;
         s_go[tid] = s.have - s.want;
@@ -231,31 +224,35 @@ __global__ __launch_bounds__(TILE) void k_kv_release(KvReleaseArgs a) {
                 a.block_table_out[e] = -1;
                 if (at < a.n_pages) a.free_list[at] = p;
             }
-        __syncthreads();
+        if (base + TILE < a.n_seq) __syncthreads();
     }
     if (gridDim.x > 1 && !last_block(a.ticket, &flag)) return;
     for (int base = 0; base < a.n_seq; base += TILE) {
-        page = 0;
-        const Rel s = release_seq(a, base, page, red);
+        if (a.n_seq > TILE) s = release_seq<TILE>(a, base, page, red);
         if (base + tid < a.n_seq) a.kv_len_out[base + tid] = s.keep;
-        __syncthreads();
     }
     if (tid == 0) *a.n_free_out = (int)min(n_free + all, (long)a.n_pages);
 }
 
 }  // namespace
 
+// One tile of sequences needs one pass of loads and sums, so the tile (and the
+// block) is as large as the batch; tokens and block tables are spread over more
+// blocks only where they outweigh the sums that every block repeats.
 int kv_plan(const KvPlanArgs& a, hipStream_t st) {
-    // one block serves a small batch without the wait for the last block
-    const int by_tok = (a.n_tok + 2047) / 2048, by_seq = (a.n_seq + 127) / 128;
-    const int grid = min(128, max(1, max(by_tok, by_seq)));
-    hipLaunchKernelGGL(k_kv_plan, dim3(grid), dim3(TILE), 0, st, a);
+    const int tile = a.n_seq <= 256 ? 256 : 1024;
+    const int by_tok = (a.n_tok + 4 * tile - 1) / (4 * tile), by_seq = (a.n_seq + 127) / 128;
+    const dim3 grid(min(256, max(1, max(by_tok, by_seq))));
+    if (tile == 256) hipLaunchKernelGGL(k_kv_plan<256>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_kv_plan<1024>, grid, dim3(1024), 0, st, a);
     return 0;
 }
 
 int kv_release(const KvReleaseArgs& a, hipStream_t st) {
-    const int grid = min(128, max(1, (a.n_seq + 31) / 32));
-    hipLaunchKernelGGL(k_kv_release, dim3(grid), dim3(TILE), 0, st, a);
+    const int tile = a.n_seq <= 256 ? 256 : 1024;
+    const dim3 grid(min(128, max(1, (a.n_seq + 15) / 16)));
+    if (tile == 256) hipLaunchKernelGGL(k_kv_release<256>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_kv_release<1024>, grid, dim3(1024), 0, st, a);
     return 0;
 }
 
