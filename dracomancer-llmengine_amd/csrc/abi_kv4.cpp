@@ -208,7 +208,7 @@ int draco_kv4_append(const DracoKv4* cache, const DracoKv4Append* p, void* strea
             return fail(-1, "%s: %d axes with positions %ld apart", who, p->n_axes, p->pos_stride);
         for (int i = 0; i < p->rot / 2; i++) {
             if (p->axis[i] >= p->n_axes) return fail(-1, "%s: pair %d is on axis %d of %d", who, i, p->axis[i], p->n_axes);
-            a.axis[i] = p->axis[i];
+            a.axis[i / 16] |= (uint32_t)p->axis[i] << (2 * (i % 16));
         }
     }
     // q_out may be q itself (each value is written by the lane that read it
@@ -228,7 +228,7 @@ int draco_kv4_append(const DracoKv4* cache, const DracoKv4Append* p, void* strea
     a.rot = p->rot;
     a.n_axes = p->n_axes;
     a.pos = p->pos;
-    a.pos_stride = p->pos_stride;
+    a.pos_stride = p->n_axes > 1 ? p->pos_stride : 0;
     a.table = p->table;
     a.table_rows = p->table_rows;
     OnDevice dev;

@@ -44,7 +44,8 @@ struct Kv4AppendArgs {
     long pos_stride;
     const float* table;  // [table_rows][rot/2][cos, sin]
     int table_rows;
-    uint8_t axis[128];   // axis of pair i
+    uint32_t axis[8];    // of pair i: bits 2 (i % 16) .. of word i / 16
+    int kv_passes;       // (filled by kv4_append)
 };
 int kv4_append(const Kv4AppendArgs& a, bool f16, bool halves, hipStream_t st);
 int kv4_read(const Kv4View& c, const int* slot, int n, float* k, float* v, hipStream_t st);

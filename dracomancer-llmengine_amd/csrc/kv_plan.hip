@@ -241,7 +241,7 @@ __global__ __launch_bounds__(TILE) void k_kv_release(KvReleaseArgs a) {
 // blocks only where they outweigh the sums that every block repeats.
 int kv_plan(const KvPlanArgs& a, hipStream_t st) {
     const int tile = a.n_seq <= 256 ? 256 : 1024;
-    const int by_tok = (a.n_tok + 4 * tile - 1) / (4 * tile), by_seq = (a.n_seq + 127) / 128;
+    const int by_tok = (a.n_tok + tile - 1) / tile, by_seq = (a.n_seq + 127) / 128;
     const dim3 grid(min(256, max(1, max(by_tok, by_seq))));
     if (tile == 256) hipLaunchKernelGGL(k_kv_plan<256>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(k_kv_plan<1024>, grid, dim3(1024), 0, st, a);

@@ -564,7 +564,7 @@ int draco_kv_release(const DracoKvRelease* p, void* stream);
  * turns by row pos[axis[i]][token] of `table` ([table_rows][rot/2] of cos,
  * sin: draco_rope_table's layout).  Text has one axis; images and video up to
  * four (time, height, width, ...), each with its own positions, pos_stride
- * ints apart.  Products and sums in 64 bits, one rounding.  A position outside
+ * ints apart.  Products and sums in 64 bits, one rounding to fp32 (f16 q: another to f16).  A position outside
  * the table makes its pairs NaN.  q_out may be q with pairing 0 or rot 0 only.
  *
  * A k or v row that is not finite is held as NaN: attention rows that see the
