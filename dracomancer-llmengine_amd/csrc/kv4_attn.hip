@@ -19,6 +19,8 @@
 // rounding).
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "dev_common.h"
 #include "kv4.h"
 #include "wave_scan.h"
@@ -415,14 +417,11 @@ __device__ __forceinline__ float row_max(const Row& w, int key, int sink, f4v c[
     return rows_reduce(top, OpMax{});
 }
 
-// Scores c (keys 16 g + 4 t + r of the unit at key0) to probabilities as the
-// second product's operands; acc follows the reference score where it moves.
-// The reference moves only when a maximum passes it by 2^PSLACK, so that most
-// units leave acc alone.
-template <bool F16, int MT>
-__device__ __forceinline__ void softmax(Row& w, bool whole, int key0, int sink, f4v c[4], f4v* acc, h8v ph[2], h8v pl[2]) {
-    const int key = key0 + 16 * ((threadIdx.x & 63) >> 4);
-    const float top = whole ? row_max<false>(w, key, sink, c) : row_max<true>(w, key, sink, c);
+// The reference follows a unit's maximum, and acc and l the reference.  It
+// moves only when a maximum passes it by 2^PSLACK, so that most units leave
+// acc alone.
+template <int MT>
+__device__ __forceinline__ void follow(Row& w, float top, f4v* acc) {
     const bool grow = top > w.m && !(w.f * (top - w.m) <= PSLACK);
     if (__any(grow)) {
         const float nfm = grow ? PBIAS - w.f * top : w.nfm;
@@ -433,6 +432,10 @@ __device__ __forceinline__ void softmax(Row& w, bool whole, int key0, int sink, 
 #pragma unroll
         for (int m = 0; m < MT; m++) acc[m] *= keep;
     }
+}
+// Scores to probabilities as the second product's operands.
+template <bool F16>
+__device__ __forceinline__ void probabilities(Row& w, const f4v c[4], h8v ph[2], h8v pl[2]) {
     float p[2][8], sum = 0.0f;
 #pragma unroll
     for (int x = 0; x < 4; x++)
@@ -445,6 +448,14 @@ __device__ __forceinline__ void softmax(Row& w, bool whole, int key0, int sink, 
     w.l += sum;
     split8<F16>(p[0], ph[0], pl[0]);
     split8<F16>(p[1], ph[1], pl[1]);
+}
+// Both, for scores of keys 16 g + 4 t + r of the unit at key0.
+template <bool F16, int MT>
+__device__ __forceinline__ void softmax(Row& w, bool whole, int key0, int sink, f4v c[4], f4v* acc, h8v ph[2], h8v pl[2]) {
+    const int key = key0 + 16 * ((threadIdx.x & 63) >> 4);
+    const float top = whole ? row_max<false>(w, key, sink, c) : row_max<true>(w, key, sink, c);
+    follow<MT>(w, top, acc);
+    probabilities<F16>(w, c, ph, pl);
 }
 
 template <bool F16>
@@ -971,6 +982,217 @@ __global__ __launch_bounds__(64 * W, HD == 256 && NT == 2 ? 1 : 2) void k_kv4_at
     join_blocks<HD, F16, R, 64 * W>(a, shares);
 }
 
+// Prompts: eight waves of 16 NT rows, one tile a block.  A SIMD overlaps
+// matrix products with vector work only where the two stand side by side in
+// the stream (waves that share operands through LDS run in step), so a turn
+// computes the exponentials of unit n among the products of unit n + 1's
+// scores, and stages later units' operands among unit n's output products.
+// K operands are staged two units ahead and V operands one; one barrier a turn.
+template <int HD, bool F16, int NT>
+__global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
+    constexpr int KS = HD / 32, MT = HD / 16, W = 8, R = 16 * NT * W;
+    constexpr int KW = 4 * KS / W;  // K words a lane stages; V parts: one, of the first 2 KS waves
+    __shared__ __align__(16) h8v s_k[2][4 * KS * 64];  // [word][key tile][lane]
+    __shared__ __align__(16) h8v s_v[2][4 * KS * 64];  // [block][part][low, high][lane]
+    const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    Tile t;
+    if (!whole_tile<R>(a, t)) return;
+    const Units u = tile_units(a, t, t.r0, t.r1);
+    const int ps = 1 << a.c.ps_shift;
+    const int kt = wave & 3, s0 = (wave >> 2) * KW;
+    const bool stage_v = wave < 2 * KS;
+    KRow<HD, KW> k;
+    VPart v;
+    int kp, vp;  // pages of the units to load next
+    bool v_ok = true;
+    auto unit_of = [&](int n) { return u.at(max(min(n, u.n - 1), 0)); };
+    auto load_k = [&](int n) {  // unit n's K codes, and the page of unit n + 1
+        bool ok;
+        const int key = k_key(unit_of(n));
+        const uint8_t* p = page_ptr(a, kp, key, t.head, ok);
+        load_krow<HD, KW>(p, ok, ps, (key & (ps - 1)) + 4 * kt, s0, k);
+        kp = page_of(a, t.table, k_key(unit_of(n + 1)));
+    };
+    auto load_v = [&](int n) {
+        const int key = v_key(unit_of(n));
+        const uint8_t* p = page_ptr(a, vp, key, t.head, v_ok);
+        load_vpart<HD>(p, ps, key & (ps - 1), (wave >> 1) & (KS - 1), wave & 1, v);
+        vp = page_of(a, t.table, v_key(unit_of(n + 1)));
+    };
+    auto stage_k = [&](int n) {
+        h8v* bk = s_k[n & 1];
+#pragma unroll
+        for (int s = 0; s < KW; s++) bk[((s0 + s) * 4 + kt) * 64 + lane] = k_operand(k.w[s], k.scale(s));
+    };
+    auto cut_v = [&](int n) {
+        const int key0 = unit_of(n) * UNIT;
+        if (key0 + UNIT > t.len || !v_ok) cut_vpart(v, key0 + 16 * g + 8 * (wave & 1), v_ok ? t.len : 0);
+    };
+    auto stage_v_ops = [&](int n) {
+        h8v* bv = s_v[n & 1];
+        h8v lo, hi;
+        v_operands(v, lo, hi);
+        if (2 * KS >= W || stage_v) {
+            bv[(wave * 2 + 0) * 64 + lane] = lo;
+            bv[(wave * 2 + 1) * 64 + lane] = hi;
+        }
+    };
+    kp = page_of(a, t.table, k_key(unit_of(0)));
+    vp = page_of(a, t.table, v_key(unit_of(0)));
+    // this wave's rows; a wave without any repeats the tile's last and stores nothing
+    const int r0 = min(t.r0 + wave * 16 * NT, t.r1 - 1), r1 = min(t.r0 + (wave + 1) * 16 * NT, t.r1);
+    h8v qh[NT][KS], ql[NT][F16 ? 1 : KS];
+    Row w[NT];
+    f4v acc[NT][MT], c[NT][4], d[NT][4];
+#pragma unroll
+    for (int x = 0; x < NT; x++) {
+        const int r = min(r0 + 16 * x + i, t.r1 - 1);
+        float f;
+        load_q<HD, F16>(a, t, r, qh[x], ql[x], f);
+        row_init(a, t, r, f, w[x]);
+#pragma unroll
+        for (int m = 0; m < MT; m++) acc[x][m] = f4v{0, 0, 0, 0};
+    }
+    const Whole whole = whole_of(a, t, r0, max(r1, r0 + 1));
+    load_k(0);
+    load_v(0);
+    stage_k(0);
+    cut_v(0);
+    stage_v_ops(0);
+    load_k(1);
+    load_v(1);
+    stage_k(1);
+    load_k(2);
+    lds_barrier();
+    // Operands are read one step ahead of their products, and each step's
+    // products have a share of the vector work between them: left to itself the
+    // compiler reads an operand where it is used and waits out the LDS.
+    h8v cur[4], nxt[4];
+    auto read = [&](const h8v* p, h8v (&o)[4]) {
+#pragma unroll
+        for (int y = 0; y < 4; y++) o[y] = p[y * 64 + lane];
+    };
+    auto products = [&](int e, f4v (&s)[NT][4]) {
+#pragma unroll
+        for (int y = 0; y < 4; y++)
+#pragma unroll
+            for (int x = 0; x < NT; x++) s[x][y] = mfma(cur[y], qh[x][e], s[x][y]);
+        if constexpr (!F16) {
+#pragma unroll
+            for (int y = 0; y < 4; y++)
+#pragma unroll
+                for (int x = 0; x < NT; x++) s[x][y] = mfma(cur[y], ql[x][e], s[x][y]);
+        }
+    };
+    auto clear = [&](f4v (&s)[NT][4]) {
+#pragma unroll
+        for (int x = 0; x < NT; x++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) s[x][y] = f4v{0, 0, 0, 0};
+    };
+    constexpr int NM = 4 * NT * (F16 ? 1 : 2);  // products of a step
+    auto interleave = [&](auto vec) {           // .. with vec.value vector instructions behind each
+#pragma unroll
+        for (int m = 0; m < NM; m++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, decltype(vec)::value, 0);
+        }
+    };
+    clear(c);
+#pragma unroll
+    for (int e = 0; e < KS; e++) {
+        read(s_k[0] + e * 256, cur);
+        products(e, c);
+    }
+    lds_barrier();  // unit 0's K buffer goes to unit 2
+    for (int n = 0; n < u.n; n++) {
+        const int key0 = u.at(n) * UNIT;
+        const bool all = whole.has(key0);
+        const h8v *bk = s_k[(n + 1) & 1], *bv = s_v[n & 1];
+        read(bk, cur);
+#pragma unroll
+        for (int x = 0; x < NT; x++) {
+            const int key = key0 + 16 * g;
+            const float top = all ? row_max<false>(w[x], key, a.sink, c[x]) : row_max<true>(w[x], key, a.sink, c[x]);
+            follow<MT>(w[x], top, acc[x]);
+        }
+        cut_v(n + 1);
+        // scores of unit n + 1, probabilities of unit n
+        h8v ph[NT][2], pl[NT][2];
+        clear(d);
+#pragma unroll
+        for (int e = 0; e < KS; e++) {
+            read(e + 1 < KS ? bk + (e + 1) * 256 : bv, nxt);
+            __builtin_amdgcn_sched_barrier(0);
+            products(e, d);
+#pragma unroll
+            for (int y = e * 4 / KS; y < (e + 1) * 4 / KS; y++)
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int z = 0; z < 4; z++) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y][z], w[x].f, w[x].nfm));
+                        const int at = 4 * (y & 1) + z;
+                        w[x].l += p;
+                        ph[x][y >> 1][at] = (_Float16)p;
+                        if constexpr (!F16) pl[x][y >> 1][at] = (_Float16)__builtin_fmaf((float)ph[x][y >> 1][at], -1.0f, p);
+                    }
+            interleave(std::integral_constant<int, 16 * NT * (F16 ? 4 : 6) / KS / NM>());
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < 4; y++) cur[y] = nxt[y];
+        }
+        // output of unit n; operands of units n + 2 and n + 1, codes of the units after them
+#pragma unroll
+        for (int b = 0; b < KS; b++) {
+            if (b + 1 < KS) read(bv + (b + 1) * 256, nxt);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+#pragma unroll
+                for (int x = 0; x < NT; x++) {
+                    acc[x][2 * b] = mfma(cur[2 * y], ph[x][y], acc[x][2 * b]);
+                    acc[x][2 * b + 1] = mfma(cur[2 * y + 1], ph[x][y], acc[x][2 * b + 1]);
+                }
+                if constexpr (!F16) {
+#pragma unroll
+                    for (int x = 0; x < NT; x++) {
+                        acc[x][2 * b] = mfma(cur[2 * y], pl[x][y], acc[x][2 * b]);
+                        acc[x][2 * b + 1] = mfma(cur[2 * y + 1], pl[x][y], acc[x][2 * b + 1]);
+                    }
+                }
+            }
+            if (b == 0) {
+                stage_k(n + 2);
+                load_k(n + 3);
+            }
+            if (b == KS / 2) {
+                stage_v_ops(n + 1);
+                load_v(n + 2);
+            }
+            interleave(std::integral_constant<int, 4>());
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < 4; y++) cur[y] = nxt[y];
+        }
+        lds_barrier();
+#pragma unroll
+        for (int x = 0; x < NT; x++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) c[x][y] = d[x][y];
+    }
+#pragma unroll
+    for (int x = 0; x < NT; x++) {
+        const float l = rows_sum(w[x].l);
+        const int r = r0 + 16 * x + i;
+        if (r >= r1) continue;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        const long at = out_at(a, t, r, HD);
+#pragma unroll
+        for (int m = 0; m < MT; m++) store4<F16>(a, at + 16 * m + 4 * g, acc[x][m] * inv);
+    }
+}
+
 template <int HD, bool F16>
 void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid);
@@ -980,7 +1202,7 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
         hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 4, 1>), grid, dim3(256), 0, st, a);
     } else {
         if constexpr (HD == 256 && F16) hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 4, 2>), grid, dim3(256), 0, st, a);
-        else if constexpr (HD != 256) hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 8, 2>), grid, dim3(512), 0, st, a);
+        else if constexpr (HD != 256) hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, (HD == 128 && !F16 ? 1 : 2)>), grid, dim3(512), 0, st, a);
     }
 }
 
@@ -988,7 +1210,7 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
 
 Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, int cus) {
     Kv4AttnPlan p = {};
-    const int group = n_head / n_kv, big = hd != 256 ? 256 : f16 ? 128 : 64;
+    const int group = n_head / n_kv, big = hd == 64 ? 256 : hd == 128 ? (f16 ? 256 : 128) : f16 ? 128 : 64;
     const long rows = (long)max_q * group;
     auto tiles = [&](int r) { return ((long)n_tok * group / r + n_seq) * n_kv; };
     p.rows = rows <= 16 ? 16 : 64;
