@@ -420,18 +420,17 @@ __device__ __forceinline__ float row_max(const Row& w, int key, int sink, f4v c[
 // The reference follows a unit's maximum, and acc and l the reference.  It
 // moves only when a maximum passes it by 2^PSLACK, so that most units leave
 // acc alone.
+__device__ __forceinline__ bool grows(const Row& w, float top) { return top > w.m && !(w.f * (top - w.m) <= PSLACK); }
 template <int MT>
-__device__ __forceinline__ void follow(Row& w, float top, f4v* acc) {
-    const bool grow = top > w.m && !(w.f * (top - w.m) <= PSLACK);
-    if (__any(grow)) {
-        const float nfm = grow ? PBIAS - w.f * top : w.nfm;
-        const float keep = !grow ? 1.0f : w.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(nfm - w.nfm);
-        if (grow) w.m = top;
-        w.nfm = nfm;
-        w.l *= keep;
+__device__ __forceinline__ float follow(Row& w, float top, f4v* acc) {  // what acc was multiplied by
+    const bool grow = grows(w, top);
+    const float nfm = grow ? PBIAS - w.f * top : w.nfm;
+    const float keep = !grow ? 1.0f : w.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(nfm - w.nfm);
+    if (grow) w.m = top;
+    w.nfm = nfm;
 #pragma unroll
-        for (int m = 0; m < MT; m++) acc[m] *= keep;
-    }
+    for (int m = 0; m < MT; m++) acc[m] *= keep;
+    return keep;
 }
 // Scores to probabilities as the second product's operands.
 template <bool F16>
@@ -454,7 +453,7 @@ template <bool F16, int MT>
 __device__ __forceinline__ void softmax(Row& w, bool whole, int key0, int sink, f4v c[4], f4v* acc, h8v ph[2], h8v pl[2]) {
     const int key = key0 + 16 * ((threadIdx.x & 63) >> 4);
     const float top = whole ? row_max<false>(w, key, sink, c) : row_max<true>(w, key, sink, c);
-    follow<MT>(w, top, acc);
+    if (__any(grows(w, top))) w.l *= follow<MT>(w, top, acc);
     probabilities<F16>(w, c, ph, pl);
 }
 
@@ -1105,16 +1104,36 @@ __global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
         products(e, c);
     }
     lds_barrier();  // unit 0's K buffer goes to unit 2
-    for (int n = 0; n < u.n; n++) {
+    // Sums of the rounded p, by products with ones (a lane's column is its row):
+    // less work than adding, and the weights that are applied sum to one.
+    f4v sum[NT];
+    h8v ones;
+#pragma unroll
+    for (int e = 0; e < 8; e++) ones[e] = (_Float16)1.0f;
+#pragma unroll
+    for (int x = 0; x < NT; x++) sum[x] = f4v{w[x].l, w[x].l, w[x].l, w[x].l};
+    auto turn = [&](int n, f4v (&c)[NT][4], f4v (&d)[NT][4]) {
         const int key0 = u.at(n) * UNIT;
         const bool all = whole.has(key0);
         const h8v *bk = s_k[(n + 1) & 1], *bv = s_v[n & 1];
         read(bk, cur);
+        float top[NT];
+        if (all) {
 #pragma unroll
-        for (int x = 0; x < NT; x++) {
-            const int key = key0 + 16 * g;
-            const float top = all ? row_max<false>(w[x], key, a.sink, c[x]) : row_max<true>(w[x], key, a.sink, c[x]);
-            follow<MT>(w[x], top, acc[x]);
+            for (int x = 0; x < NT; x++) top[x] = row_max<false>(w[x], key0 + 16 * g, a.sink, c[x]);
+        } else {
+#pragma unroll
+            for (int x = 0; x < NT; x++) top[x] = row_max<true>(w[x], key0 + 16 * g, a.sink, c[x]);
+        }
+        bool grow = false;
+#pragma unroll
+        for (int x = 0; x < NT; x++) grow |= grows(w[x], top[x]);
+        if (__any(grow)) {
+#pragma unroll
+            for (int x = 0; x < NT; x++) {
+                const float keep = follow<MT>(w[x], top[x], acc[x]);
+                sum[x] *= keep;
+            }
         }
         cut_v(n + 1);
         // scores of unit n + 1, probabilities of unit n
@@ -1133,11 +1152,10 @@ __global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
                     for (int z = 0; z < 4; z++) {
                         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y][z], w[x].f, w[x].nfm));
                         const int at = 4 * (y & 1) + z;
-                        w[x].l += p;
                         ph[x][y >> 1][at] = (_Float16)p;
                         if constexpr (!F16) pl[x][y >> 1][at] = (_Float16)__builtin_fmaf((float)ph[x][y >> 1][at], -1.0f, p);
                     }
-            interleave(std::integral_constant<int, 16 * NT * (F16 ? 4 : 6) / KS / NM>());
+            interleave(std::integral_constant<int, 16 * NT * (F16 ? 3 : 5) / KS / NM>());
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int y = 0; y < 4; y++) cur[y] = nxt[y];
@@ -1170,20 +1188,29 @@ __global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
                 stage_v_ops(n + 1);
                 load_v(n + 2);
             }
+            if (b == KS - 1) {
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        sum[x] = mfma(ones, ph[x][y], sum[x]);
+                        if constexpr (!F16) sum[x] = mfma(ones, pl[x][y], sum[x]);
+                    }
+            }
             interleave(std::integral_constant<int, 4>());
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int y = 0; y < 4; y++) cur[y] = nxt[y];
         }
         lds_barrier();
-#pragma unroll
-        for (int x = 0; x < NT; x++)
-#pragma unroll
-            for (int y = 0; y < 4; y++) c[x][y] = d[x][y];
+    };
+    for (int n = 0; n < u.n; n += 2) {  // (two turns: the scores change places without copies)
+        turn(n, c, d);
+        if (n + 1 < u.n) turn(n + 1, d, c);
     }
 #pragma unroll
     for (int x = 0; x < NT; x++) {
-        const float l = rows_sum(w[x].l);
+        const float l = sum[x][0];
         const int r = r0 + 16 * x + i;
         if (r >= r1) continue;
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
