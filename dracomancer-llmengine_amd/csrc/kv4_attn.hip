@@ -121,10 +121,12 @@ __device__ __forceinline__ Units tile_units(const Kv4AttnArgs& a, const Tile& t,
 }
 
 // The batch's work, laid out as one list of units: sequences, their tiles of R
-// rows, KV heads, units of keys (at least one each, so that every row is
-// written).  The grid's blocks take equal stretches of it, whatever the
-// lengths are: `chunk` units from `at`.  Lengths come from device memory, so
-// every wave adds them up itself, 64 sequences at a time.
+// rows, KV heads, units of keys.  A sequence's tiles all count as many units as
+// any of them may have, at least one (a tile's place is then a division away;
+// what is too much comes out as empty pieces).  The grid's blocks take equal
+// stretches of the list, whatever the lengths are: `chunk` units from `at`.
+// Lengths come from device memory, so every wave adds them up itself, 64
+// sequences at a time.
 struct Work {
     long at;      // this block's next unit
     int left;     // units left to it
@@ -132,26 +134,34 @@ struct Work {
     long rem;     // `at` within sequence `seq`
     int seq;
 };
-// Units of this lane's sequence.
+// Units that a tile of the sequence has at most.
 template <int R>
-__device__ __forceinline__ long batch_units(const Kv4AttnArgs& a, const Batch& b) {
+__device__ __forceinline__ int tile_bound(const Kv4AttnArgs& a, const Tile& t) {
+    const long last = (long)t.len - 1;  // (the last row's position, behind no key)
+    long n = last < 0 || t.rows == 0 ? 0 : last / UNIT + 1;
+    if (a.window > 0) {
+        const long span = (long)a.window + (R + a.group - 2) / a.group;  // keys under the windows of R rows
+        n = min(n, (span + UNIT - 2) / UNIT + 1 + ((long)a.sink + UNIT - 1) / UNIT);
+    }
+    return (int)max(n, 1L);
+}
+template <int R>
+__device__ __forceinline__ long batch_units(const Kv4AttnArgs& a, const Batch& b) {  // of this lane's sequence
     if (b.base + ((int)threadIdx.x & 63) >= a.n_seq) return 0;
     Tile t;
     tile_of(a, b.q0, b.q1, b.len, t);
-    long n = 0;
-    for (int r = 0; r < t.rows; r += R) n += max(tile_units(a, t, r, min(r + R, t.rows)).n, 1);
-    return n * a.c.n_kv;
+    return (long)((t.rows + R - 1) / R) * tile_bound<R>(a, t) * a.c.n_kv;
 }
 template <int R>
-__device__ __forceinline__ bool work_of(const Kv4AttnArgs& a, Work& w, Batch& b) {
+__device__ __forceinline__ bool work_of(const Kv4AttnArgs& a, Work& w, Batch& b, int block, int blocks) {
     batch_of(a, 0, b);
     long mine = wave_scan(batch_units<R>(a, b)), total = lane_of(mine, 63);
     for (int s = 64; s < a.n_seq; s += 64) {
         batch_of(a, s, b);
         total += lane_of(wave_scan(batch_units<R>(a, b)), 63);
     }
-    w.chunk = max(a.chunk, (int)((total + gridDim.x - 1) / gridDim.x));
-    w.at = (long)blockIdx.x * w.chunk;
+    w.chunk = max(a.chunk, (int)((total + blocks - 1) / blocks));
+    w.at = (long)block * w.chunk;
     w.left = (int)min((long)w.chunk, total - w.at);
     if (w.left <= 0) return false;
     long before = 0;
@@ -208,29 +218,31 @@ struct Piece {
 };
 template <int R>
 __device__ __forceinline__ void piece_of(const Kv4AttnArgs& a, Work& w, Batch& b, Tile& t, Units& u, Piece& p) {
-    for (;;) {
+    for (;; w.seq++) {
         seq_of(a, b, w.seq, t);
-        long rem = w.rem;
-        for (t.r0 = 0; t.r0 < t.rows; t.r0 += R) {
-            t.r1 = min(t.r0 + R, t.rows);
-            u = tile_units(a, t, t.r0, t.r1);
-            p.n = max(u.n, 1);
-            if (rem < (long)p.n * a.c.n_kv) {
-                for (t.head = 0; rem >= p.n; t.head++) rem -= p.n;
-                p.lo = (int)rem;
-                p.hi = min(p.lo + w.left, p.n);
-                p.first = w.at - p.lo;
-                const int took = p.hi - p.lo;
-                w.at += took;
-                w.rem += took;
-                w.left -= took;
-                p.hi = min(p.hi, u.n);
-                return;
-            }
-            rem -= (long)p.n * a.c.n_kv;
+        p.n = uni(tile_bound<R>(a, t));
+        const long tile = (long)p.n * a.c.n_kv, all = (t.rows + R - 1) / R * tile;
+        if (w.rem >= all) {  // (its rows are done; `left` says that more follow)
+            w.rem -= all;
+            continue;
         }
-        w.rem = rem;
-        w.seq++;  // (its rows are done; `left` says that more follow)
+        long rem = w.rem;
+        const int k = rem < tile ? 0 : (int)((unsigned long)rem / (unsigned long)tile);
+        rem -= k * tile;
+        for (t.head = 0; rem >= p.n; t.head++) rem -= p.n;
+        t.r0 = k * R;
+        t.r1 = min(t.r0 + R, t.rows);
+        u = tile_units(a, t, t.r0, t.r1);
+        p.lo = (int)rem;
+        p.hi = min(p.lo + w.left, p.n);
+        p.first = w.at - p.lo;
+        const int took = p.hi - p.lo;
+        w.at += took;
+        w.rem += took;
+        w.left -= took;
+        p.lo = min(p.lo, u.n);
+        p.hi = min(p.hi, u.n);
+        return;
     }
 }
 
@@ -647,7 +659,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
     const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     Work work;
     Batch batch;
-    if (!work_of<16>(a, work, batch)) return;
+    if (!work_of<16>(a, work, batch, blockIdx.x, gridDim.x)) return;
     const int ps = 1 << a.c.ps_shift;
     Tile t;
     Units u;
@@ -814,11 +826,10 @@ __global__ __launch_bounds__(64 * W, HD == 256 && NT == 2 ? 1 : 2) void k_kv4_at
     if (a.whole) {
         if (!whole_tile<R>(a, t)) return;
         work.left = 0;
-    } else if (!work_of<R>(a, work, batch)) {
+    } else if (!work_of<R>(a, work, batch, blockIdx.x, gridDim.x)) {
         return;
     }
     const int ps = 1 << a.c.ps_shift;
-    Shares shares;
   do {
     Units u;
     Piece part;
@@ -969,42 +980,62 @@ __global__ __launch_bounds__(64 * W, HD == 256 && NT == 2 ? 1 : 2) void k_kv4_at
 #pragma unroll
             for (int m = 0; m < MT; m++) store4<F16>(a, at + 16 * m + 4 * g, acc[x][m] * inv);
         } else {
-            const Parts parts = parts_of(a);
-            const unsigned row = part_at<HD, R>(sh.slot(blockIdx.x), r - t.r0);
+            float* row = a.part + part_at<HD, R>(sh.slot(blockIdx.x), r - t.r0);
 #pragma unroll
-            for (int m = 0; m < MT; m++) parts.put4(row + 16 * m + 4 * g, acc[x][m]);
-            if (g == 0) parts.put4(row + HD, f4v{l, w[x].nfm, 0, 0});
+            for (int m = 0; m < MT; m++) *(f4v*)(row + 16 * m + 4 * g) = acc[x][m];
+            if (g == 0) *(f4v*)(row + HD) = f4v{l, w[x].nfm, 0, 0};
         }
     }
-    if (sh.split()) shares.add(sh, t);
   } while (work.left > 0);
-    join_blocks<HD, F16, R, 64 * W>(a, shares);
 }
 
-// Prompts: eight waves of 16 NT rows, one tile a block.  A SIMD overlaps
-// matrix products with vector work only where the two stand side by side in
-// the stream (waves that share operands through LDS run in step), so a turn
-// computes the exponentials of unit n among the products of unit n + 1's
-// scores, and stages later units' operands among unit n's output products.
-// K operands are staged two units ahead and V operands one; one barrier a turn.
-template <int HD, bool F16, int NT>
-__global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
-    constexpr int KS = HD / 32, MT = HD / 16, W = 8, R = 16 * NT * W;
-    constexpr int KW = 4 * KS / W;  // K words a lane stages; V parts: one, of the first 2 KS waves
+// More rows (drafts, prompts): W waves of 16 NT rows over the same units, whose
+// codes they turn into f16 operands in LDS together, in the order in which a
+// lane reads them (16 bytes a lane, no bank conflict).  A SIMD overlaps matrix
+// products with vector work only where the two stand side by side in the
+// stream (waves that share operands run in step), so a turn computes the
+// exponentials of unit n among the products of unit n + 1's scores, and stages
+// later units' operands among unit n's output products.  K operands are staged
+// two units ahead and V operands one; one barrier a turn.
+template <int HD, bool F16, int W, int NT, bool SPLIT>
+__global__ __launch_bounds__(64 * W, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
+    constexpr int KS = HD / 32, MT = HD / 16, R = 16 * NT * W;
+    constexpr int KW = 4 * KS / W;                    // K words a lane stages
+    constexpr int NJ = 2 * KS >= W ? 2 * KS / W : 1;  // V parts a lane stages (HD 64, 8 waves: the first 4)
     __shared__ __align__(16) h8v s_k[2][4 * KS * 64];  // [word][key tile][lane]
     __shared__ __align__(16) h8v s_v[2][4 * KS * 64];  // [block][part][low, high][lane]
     const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    Work work;
+    Batch batch;
     Tile t;
-    if (!whole_tile<R>(a, t)) return;
-    const Units u = tile_units(a, t, t.r0, t.r1);
+    const bool one = !SPLIT || a.whole;
+    if (one) {
+        if (!whole_tile<R>(a, t)) return;
+        work.left = 0;
+    } else if constexpr (SPLIT) {
+        if (!work_of<R>(a, work, batch, blockIdx.x, gridDim.x)) return;
+    }
     const int ps = 1 << a.c.ps_shift;
-    const int kt = wave & 3, s0 = (wave >> 2) * KW;
-    const bool stage_v = wave < 2 * KS;
+    const int kt = wave & 3, s0 = W == 8 ? (wave >> 2) * KW : 0, j0 = wave * NJ;
+    const bool stage_v = j0 < 2 * KS;
+  do {
+    Units u;
+    Piece part;
+    if (one) {
+        u = tile_units(a, t, t.r0, t.r1);
+        part.lo = 0;
+        part.hi = u.n;
+    } else if constexpr (SPLIT) {
+        piece_of<R>(a, work, batch, t, u, part);
+    }
+    const int units = part.hi - part.lo;
+    __syncthreads();  // the last piece's operands are read
     KRow<HD, KW> k;
-    VPart v;
+    VPart v[NJ];
     int kp, vp;  // pages of the units to load next
     bool v_ok = true;
-    auto unit_of = [&](int n) { return u.at(max(min(n, u.n - 1), 0)); };
+    // (past the end the last unit again: no branch around loads)
+    auto unit_of = [&](int n) { return u.at(max(min(part.lo + n, part.hi - 1), 0)); };
     auto load_k = [&](int n) {  // unit n's K codes, and the page of unit n + 1
         bool ok;
         const int key = k_key(unit_of(n));
@@ -1015,7 +1046,8 @@ __global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
     auto load_v = [&](int n) {
         const int key = v_key(unit_of(n));
         const uint8_t* p = page_ptr(a, vp, key, t.head, v_ok);
-        load_vpart<HD>(p, ps, key & (ps - 1), (wave >> 1) & (KS - 1), wave & 1, v);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) load_vpart<HD>(p, ps, key & (ps - 1), ((j0 + j) >> 1) & (KS - 1), (j0 + j) & 1, v[j]);
         vp = page_of(a, t.table, v_key(unit_of(n + 1)));
     };
     auto stage_k = [&](int n) {
@@ -1025,15 +1057,21 @@ __global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
     };
     auto cut_v = [&](int n) {
         const int key0 = unit_of(n) * UNIT;
-        if (key0 + UNIT > t.len || !v_ok) cut_vpart(v, key0 + 16 * g + 8 * (wave & 1), v_ok ? t.len : 0);
+        if (key0 + UNIT > t.len || !v_ok) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) cut_vpart(v[j], key0 + 16 * g + 8 * ((j0 + j) & 1), v_ok ? t.len : 0);
+        }
     };
     auto stage_v_ops = [&](int n) {
         h8v* bv = s_v[n & 1];
-        h8v lo, hi;
-        v_operands(v, lo, hi);
-        if (2 * KS >= W || stage_v) {
-            bv[(wave * 2 + 0) * 64 + lane] = lo;
-            bv[(wave * 2 + 1) * 64 + lane] = hi;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            h8v lo, hi;
+            v_operands(v[j], lo, hi);
+            if (2 * KS >= W || stage_v) {
+                bv[((j0 + j) * 2 + 0) * 64 + lane] = lo;
+                bv[((j0 + j) * 2 + 1) * 64 + lane] = hi;
+            }
         }
     };
     kp = page_of(a, t.table, k_key(unit_of(0)));
@@ -1113,7 +1151,7 @@ __global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
 #pragma unroll
     for (int x = 0; x < NT; x++) sum[x] = f4v{w[x].l, w[x].l, w[x].l, w[x].l};
     auto turn = [&](int n, f4v (&c)[NT][4], f4v (&d)[NT][4]) {
-        const int key0 = u.at(n) * UNIT;
+        const int key0 = unit_of(n) * UNIT;
         const bool all = whole.has(key0);
         const h8v *bk = s_k[(n + 1) & 1], *bv = s_v[n & 1];
         read(bk, cur);
@@ -1204,46 +1242,109 @@ __global__ __launch_bounds__(512, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
         }
         lds_barrier();
     };
-    for (int n = 0; n < u.n; n += 2) {  // (two turns: the scores change places without copies)
+    for (int n = 0; n < units; n += 2) {  // (two turns: the scores change places without copies)
         turn(n, c, d);
-        if (n + 1 < u.n) turn(n + 1, d, c);
+        if (n + 1 < units) turn(n + 1, d, c);
     }
+    const Shared sh = one ? Shared{0, 0} : shared_of(work, part);
 #pragma unroll
     for (int x = 0; x < NT; x++) {
         const float l = sum[x][0];
         const int r = r0 + 16 * x + i;
         if (r >= r1) continue;
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        const long at = out_at(a, t, r, HD);
+        if (!sh.split()) {
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+            const long at = out_at(a, t, r, HD);
 #pragma unroll
-        for (int m = 0; m < MT; m++) store4<F16>(a, at + 16 * m + 4 * g, acc[x][m] * inv);
+            for (int m = 0; m < MT; m++) store4<F16>(a, at + 16 * m + 4 * g, acc[x][m] * inv);
+        } else {
+            float* row = a.part + part_at<HD, R>(sh.slot(blockIdx.x), r - t.r0);
+#pragma unroll
+            for (int m = 0; m < MT; m++) *(f4v*)(row + 16 * m + 4 * g) = acc[x][m];
+            if (g == 0) *(f4v*)(row + HD) = f4v{l, w[x].nfm, 0, 0};
+        }
+    }
+  } while (SPLIT && work.left > 0);
+}
+
+// The shared tiles of 64 rows to one, in a launch of its own: block (b, s) has
+// 16 rows of the tile that block b of `blocks` left unfinished, if it was the
+// first on it.  (By the block that finishes last, as above, one block read all
+// parts of 64 rows: 16 rows a sequence of 9000 keys, 8 sequences, 64 us.)
+template <int HD, bool F16, int R>
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a, int blocks) {
+    constexpr int LPR = HD / 4, RPB = 256 / LPR, PB = 4;
+    Work work;
+    Batch batch;
+    if (!work_of<R>(a, work, batch, blockIdx.x, blocks)) return;
+    Tile t;
+    Units u;
+    Piece part;
+    do piece_of<R>(a, work, batch, t, u, part);
+    while (work.left > 0);
+    const Shared sh = shared_of(work, part);
+    if (!sh.split() || sh.b0 != (int)blockIdx.x) return;
+    const int l = threadIdx.x % LPR, r1 = min(t.r1, t.r0 + (int)(blockIdx.y + 1) * 16);
+    for (int r = t.r0 + (int)blockIdx.y * 16 + threadIdx.x / LPR; r < r1; r += RPB) {
+        float m = __builtin_inff(), sum = 0.0f;
+        f4v o = {0, 0, 0, 0};
+        for (int b = sh.b0; b <= sh.b1; b += PB) {
+            f4v n[PB], v[PB];
+#pragma unroll
+            for (int y = 0; y < PB; y++) {
+                const float* q = a.part + part_at<HD, R>(sh.slot(min(b + y, sh.b1)), r - t.r0);
+                n[y] = *(const f4v*)(q + HD);
+                v[y] = *(const f4v*)(q + 4 * l);
+            }
+#pragma unroll
+            for (int y = 0; y < PB; y++) {
+                if (b + y > sh.b1 || n[y].x == 0.0f) continue;  // (no key seen)
+                const float now = fminf(m, n[y].y), keep = sum != 0.0f ? __builtin_amdgcn_exp2f(now - m) : 0.0f;
+                const float w = __builtin_amdgcn_exp2f(now - n[y].y);
+                m = now;
+                sum = sum * keep + w * n[y].x;
+                o = o * keep + v[y] * w;
+            }
+        }
+        store4<F16>(a, out_at(a, t, r, HD) + 4 * l, o * (sum != 0.0f ? 1.0f / sum : 0.0f));
     }
 }
 
 template <int HD, bool F16>
 void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid);
-    if (p.rows == 16) {
-        hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, HD == 256 ? 2 : 1>), grid, dim3(256), 0, st, a);
-    } else if (p.rows == 64) {
-        hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 4, 1>), grid, dim3(256), 0, st, a);
+    if (p.rows == 16) hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, HD == 256 ? 2 : 1>), grid, dim3(256), 0, st, a);
+    else if constexpr (HD == 256) {
+        if (p.rows == 64) hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 4, 1>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 8, 1, false>), grid, dim3(512), 0, st, a);
     } else {
-        if constexpr (HD == 256 && F16) hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 4, 2>), grid, dim3(256), 0, st, a);
-        else if constexpr (HD != 256) hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, (HD == 128 && !F16 ? 1 : 2)>), grid, dim3(512), 0, st, a);
+        constexpr int NT = HD == 128 && !F16 ? 1 : 2;
+        if (p.rows == 64) hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 4, 1, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 8, NT, false>), grid, dim3(512), 0, st, a);
     }
+    if (p.rows == 64 && !p.whole)
+        hipLaunchKernelGGL((k_kv4_join<HD, F16, 64>), dim3((unsigned)p.grid, 4), dim3(256), 0, st, a, (int)p.grid);
 }
 
 }  // namespace
 
+#ifndef BIGMIN
+#define BIGMIN 1
+#endif
+#ifndef WHOLEMIN
+#define WHOLEMIN 1
+#endif
+#ifndef SPLITG
+#define SPLITG 2
+#endif
 Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, int cus) {
     Kv4AttnPlan p = {};
-    const int group = n_head / n_kv, big = hd == 64 ? 256 : hd == 128 ? (f16 ? 256 : 128) : f16 ? 128 : 64;
+    const int group = n_head / n_kv, big = hd == 64 || (hd == 128 && f16) ? 256 : 128;
     const long rows = (long)max_q * group;
-    auto tiles = [&](int r) { return ((long)n_tok * group / r + n_seq) * n_kv; };
-    p.rows = rows <= 16 ? 16 : 64;
-    if (rows > 64 && (long)n_tok * group / big * n_kv >= cus / 2) p.rows = big;
-    p.whole = rows > 16 && (long)n_tok * group / p.rows * n_kv >= cus / 2;
-    p.grid = p.whole ? tiles(p.rows) : (p.rows == 16 && hd != 256 ? 2 : 1) * cus;
+    auto tiles = [&](int r) { return (long)n_tok * group / r * n_kv; };
+    p.rows = rows <= 16 ? 16 : rows > 64 && tiles(big) >= BIGMIN * cus ? big : 64;
+    p.whole = rows > 16 && (p.rows == big || tiles(p.rows) >= WHOLEMIN * cus);
+    p.grid = p.whole ? ((long)n_tok * group / p.rows + n_seq) * n_kv : (p.rows == 16 ? (hd != 256 ? 2 : 1) : hd != 256 ? SPLITG : 1) * cus;
     p.chunk = p.rows == 16 ? 4 : 2;
     p.part_bytes = p.whole ? 0 : (size_t)p.grid * 2 * p.rows * (hd + 4) * sizeof(float);
     p.work = p.whole ? 0 : KV4_COUNT_BYTES + p.part_bytes;
