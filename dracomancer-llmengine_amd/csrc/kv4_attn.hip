@@ -806,189 +806,6 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
     join_blocks<HD, F16, 16, 64 * W>(a, shares);
 }
 
-// More rows (drafts, prompts): W waves with 16 NT rows each, over the same
-// units.  Each wave turns its share of a unit's codes into f16 operands in
-// LDS, in the order in which a lane reads them (16 bytes a lane, no bank
-// conflict), one unit ahead of their use where two buffers fit; the next
-// unit's codes are in flight meanwhile (the barrier orders LDS only).
-template <int HD, bool F16, int W, int NT>
-__global__ __launch_bounds__(64 * W, HD == 256 && NT == 2 ? 1 : 2) void k_kv4_attn_chunk(Kv4AttnArgs a) {
-    constexpr int KS = HD / 32, MT = HD / 16, R = 16 * NT * W;
-    constexpr int KW = 4 * KS / W;                   // K words a lane stages
-    constexpr int NJ = 2 * KS >= W ? 2 * KS / W : 1;  // V parts a lane stages (HD 64, 8 waves: the first 4)
-    constexpr int BUFS = HD == 256 ? 1 : 2;
-    __shared__ __align__(16) h8v s_k[BUFS][4 * KS * 64];  // [word][key tile][lane]
-    __shared__ __align__(16) h8v s_v[BUFS][4 * KS * 64];  // [block][part][low, high][lane]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    Work work;
-    Batch batch;
-    Tile t;
-    if (a.whole) {
-        if (!whole_tile<R>(a, t)) return;
-        work.left = 0;
-    } else if (!work_of<R>(a, work, batch, blockIdx.x, gridDim.x)) {
-        return;
-    }
-    const int ps = 1 << a.c.ps_shift;
-  do {
-    Units u;
-    Piece part;
-    if (a.whole) {
-        u = tile_units(a, t, t.r0, t.r1);
-        part.lo = 0;
-        part.hi = u.n;
-    } else {
-        piece_of<R>(a, work, batch, t, u, part);
-    }
-    __syncthreads();  // the last piece's operands are read
-    const int head = t.head;
-    const int kt = wave & 3, s0 = W == 8 ? (wave >> 2) * KW : 0, j0 = wave * NJ;
-    const bool stage_v = j0 < 2 * KS;
-    KRow<HD, KW> k;
-    VPart v[NJ];
-    int kp = 0, vp = 0;
-    auto unit_of = [&](int n) { return u.at(max(min(n, part.hi - 1), 0)); };  // (as above: no branch around loads)
-    auto pages = [&](int n) {
-        kp = page_of(a, t.table, k_key(unit_of(n)));
-        vp = page_of(a, t.table, v_key(unit_of(n)));
-    };
-    bool v_ok = true;
-    auto load = [&](int n) {
-        bool ok;
-        const int unit = unit_of(n);
-        const uint8_t* p = page_ptr(a, kp, k_key(unit), head, ok);
-        load_krow<HD, KW>(p, ok, ps, (k_key(unit) & (ps - 1)) + 4 * kt, s0, k);
-        if (stage_v) {
-            p = page_ptr(a, vp, v_key(unit), head, v_ok);
-#pragma unroll
-            for (int j = 0; j < NJ; j++) load_vpart<HD>(p, ps, v_key(unit) & (ps - 1), (j0 + j) >> 1, (j0 + j) & 1, v[j]);
-        }
-    };
-    pages(part.lo);
-    // this wave's rows; a wave without any repeats the tile's last and stores nothing
-    const int r0 = min(t.r0 + wave * 16 * NT, t.r1 - 1), r1 = min(t.r0 + (wave + 1) * 16 * NT, t.r1);
-    h8v qh[NT][KS], ql[NT][F16 ? 1 : KS];
-    Row w[NT];
-    f4v acc[NT][MT];
-#pragma unroll
-    for (int x = 0; x < NT; x++) {
-        const int r = min(r0 + 16 * x + i, t.r1 - 1);
-        float f;
-        load_q<HD, F16>(a, t, r, qh[x], ql[x], f);
-        row_init(a, t, r, f, w[x]);
-#pragma unroll
-        for (int m = 0; m < MT; m++) acc[x][m] = f4v{0, 0, 0, 0};
-    }
-    load(part.lo);
-    pages(part.lo + 1);
-    const Whole whole = whole_of(a, t, r0, max(r1, r0 + 1));
-    const int first_lo = a.window > 0 ? (int)max(0L, t.pos0 + r0 / a.group - a.window + 1) : 0;
-    const int last_hi = (int)(t.pos0 + (max(r1, r0 + 1) - 1) / a.group);
-    for (int n = part.lo; n < part.hi; n++) {
-        const int key0 = u.at(n) * UNIT;
-        h8v* bk = s_k[BUFS == 2 ? (n - part.lo) & 1 : 0];
-        h8v* bv = s_v[BUFS == 2 ? (n - part.lo) & 1 : 0];
-        if constexpr (BUFS == 1) lds_barrier();  // the last unit's readers are done
-#pragma unroll
-        for (int s = 0; s < KW; s++) bk[((s0 + s) * 4 + kt) * 64 + lane] = k_operand(k.w[s], k.scale(s));
-        if (stage_v) {
-            if (key0 + UNIT > t.len || !v_ok) {
-#pragma unroll
-                for (int j = 0; j < NJ; j++) cut_vpart(v[j], key0 + 16 * g + 8 * ((j0 + j) & 1), v_ok ? t.len : 0);
-            }
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                h8v lo, hi;
-                v_operands(v[j], lo, hi);
-                bv[((j0 + j) * 2 + 0) * 64 + lane] = lo;
-                bv[((j0 + j) * 2 + 1) * 64 + lane] = hi;
-            }
-        }
-        load(n + 1);
-        pages(n + 2);
-        lds_barrier();
-        // nothing here for this wave's rows: no query of it sees a key of the unit
-        if (r1 <= r0 || key0 > last_hi || (key0 + UNIT <= first_lo && key0 >= a.sink)) continue;
-        f4v c[NT][4];
-#pragma unroll
-        for (int x = 0; x < NT; x++)
-#pragma unroll
-            for (int y = 0; y < 4; y++) c[x][y] = f4v{0, 0, 0, 0};
-        // Operands are read one step ahead of their products (the fences keep
-        // them there: read where they are used, every pair waits out the LDS).
-        h8v cur[4], nxt[4];
-#pragma unroll
-        for (int y = 0; y < 4; y++) cur[y] = bk[y * 64 + lane];
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-#pragma unroll
-            for (int y = 0; y < 4; y++) nxt[y] = s + 1 < KS ? bk[((s + 1) * 4 + y) * 64 + lane] : bv[y * 64 + lane];
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < 4; y++)
-#pragma unroll
-                for (int x = 0; x < NT; x++) c[x][y] = mfma(cur[y], qh[x][s], c[x][y]);
-            if constexpr (!F16) {
-#pragma unroll
-                for (int y = 0; y < 4; y++)
-#pragma unroll
-                    for (int x = 0; x < NT; x++) c[x][y] = mfma(cur[y], ql[x][s], c[x][y]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < 4; y++) cur[y] = nxt[y];
-        }
-        h8v ph[NT][2], pl[NT][2];
-#pragma unroll
-        for (int x = 0; x < NT; x++) softmax<F16, MT>(w[x], whole.has(key0), key0, a.sink, c[x], acc[x], ph[x], pl[x]);
-#pragma unroll
-        for (int b = 0; b < KS; b++) {  // cur: tokens 0-7 low, high nibbles' dims, tokens 8-15
-            if (b + 1 < KS) {
-#pragma unroll
-                for (int y = 0; y < 4; y++) nxt[y] = bv[((b + 1) * 4 + y) * 64 + lane];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-#pragma unroll
-                for (int x = 0; x < NT; x++) {
-                    acc[x][2 * b] = mfma(cur[2 * y], ph[x][y], acc[x][2 * b]);
-                    acc[x][2 * b + 1] = mfma(cur[2 * y + 1], ph[x][y], acc[x][2 * b + 1]);
-                }
-                if constexpr (!F16) {
-#pragma unroll
-                    for (int x = 0; x < NT; x++) {
-                        acc[x][2 * b] = mfma(cur[2 * y], pl[x][y], acc[x][2 * b]);
-                        acc[x][2 * b + 1] = mfma(cur[2 * y + 1], pl[x][y], acc[x][2 * b + 1]);
-                    }
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < 4; y++) cur[y] = nxt[y];
-        }
-    }
-    const Shared sh = a.whole ? Shared{0, 0} : shared_of(work, part);
-#pragma unroll
-    for (int x = 0; x < NT; x++) {
-        const float l = rows_sum(w[x].l);
-        const int r = r0 + 16 * x + i;
-        if (r >= r1) continue;
-        if (!sh.split()) {
-            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-            const long at = out_at(a, t, r, HD);
-#pragma unroll
-            for (int m = 0; m < MT; m++) store4<F16>(a, at + 16 * m + 4 * g, acc[x][m] * inv);
-        } else {
-            float* row = a.part + part_at<HD, R>(sh.slot(blockIdx.x), r - t.r0);
-#pragma unroll
-            for (int m = 0; m < MT; m++) *(f4v*)(row + 16 * m + 4 * g) = acc[x][m];
-            if (g == 0) *(f4v*)(row + HD) = f4v{l, w[x].nfm, 0, 0};
-        }
-    }
-  } while (work.left > 0);
-}
-
 // More rows (drafts, prompts): W waves of 16 NT rows over the same units, whose
 // codes they turn into f16 operands in LDS together, in the order in which a
 // lane reads them (16 bytes a lane, no bank conflict).  A SIMD overlaps matrix
@@ -998,7 +815,7 @@ __global__ __launch_bounds__(64 * W, HD == 256 && NT == 2 ? 1 : 2) void k_kv4_at
 // later units' operands among unit n's output products.  K operands are staged
 // two units ahead and V operands one; one barrier a turn.
 template <int HD, bool F16, int W, int NT, bool SPLIT>
-__global__ __launch_bounds__(64 * W, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
     constexpr int KS = HD / 32, MT = HD / 16, R = 16 * NT * W;
     constexpr int KW = 4 * KS / W;                    // K words a lane stages
     constexpr int NJ = 2 * KS >= W ? 2 * KS / W : 1;  // V parts a lane stages (HD 64, 8 waves: the first 4)
@@ -1268,12 +1085,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
 }
 
 // The shared tiles of 64 rows to one, in a launch of its own: block (b, s) has
-// 16 rows of the tile that block b of `blocks` left unfinished, if it was the
-// first on it.  (By the block that finishes last, as above, one block read all
+// some rows of the tile that block b of `blocks` left unfinished, if it was the
+// first on it, one a lane group.  (By the block that finishes last, as above, one block read all
 // parts of 64 rows: 16 rows a sequence of 9000 keys, 8 sequences, 64 us.)
 template <int HD, bool F16, int R>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a, int blocks) {
-    constexpr int LPR = HD / 4, RPB = 256 / LPR, PB = 4;
+    constexpr int LPR = HD / 4, RPB = 256 / LPR, PB = 8;  // (eight blocks' parts in flight)
     Work work;
     Batch batch;
     if (!work_of<R>(a, work, batch, blockIdx.x, blocks)) return;
@@ -1284,8 +1101,8 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a, int blocks) {
     while (work.left > 0);
     const Shared sh = shared_of(work, part);
     if (!sh.split() || sh.b0 != (int)blockIdx.x) return;
-    const int l = threadIdx.x % LPR, r1 = min(t.r1, t.r0 + (int)(blockIdx.y + 1) * 16);
-    for (int r = t.r0 + (int)blockIdx.y * 16 + threadIdx.x / LPR; r < r1; r += RPB) {
+    const int l = threadIdx.x % LPR, r = t.r0 + (int)blockIdx.y * RPB + threadIdx.x / LPR;
+    if (r < t.r1) {
         float m = __builtin_inff(), sum = 0.0f;
         f4v o = {0, 0, 0, 0};
         for (int b = sh.b0; b <= sh.b1; b += PB) {
@@ -1313,39 +1130,46 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a, int blocks) {
 template <int HD, bool F16>
 void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid);
-    if (p.rows == 16) hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, HD == 256 ? 2 : 1>), grid, dim3(256), 0, st, a);
-    else if constexpr (HD == 256) {
-        if (p.rows == 64) hipLaunchKernelGGL((k_kv4_attn_chunk<HD, F16, 4, 1>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 8, 1, false>), grid, dim3(512), 0, st, a);
-    } else {
-        constexpr int NT = HD == 128 && !F16 ? 1 : 2;
-        if (p.rows == 64) hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 4, 1, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 8, NT, false>), grid, dim3(512), 0, st, a);
+    constexpr int NT = HD == 64 || (HD == 128 && F16) ? 2 : 1;  // row tiles a wave of the large tiles
+    if (p.rows == 16) {
+        hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, HD == 256 ? 2 : 1>), grid, dim3(256), 0, st, a);
+    } else if (p.rows == 64) {
+        hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 4, 1, true>), grid, dim3(256), 0, st, a);
+        if (p.whole) return;
+        constexpr int RPB = 256 / (HD / 4);
+        hipLaunchKernelGGL((k_kv4_join<HD, F16, 64>), dim3((unsigned)p.grid, 64 / RPB), dim3(256), 0, st, a, (int)p.grid);
+    } else if constexpr (HD != 256 || F16) {
+        hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 8, NT, false>), grid, dim3(512), 0, st, a);
     }
-    if (p.rows == 64 && !p.whole)
-        hipLaunchKernelGGL((k_kv4_join<HD, F16, 64>), dim3((unsigned)p.grid, 4), dim3(256), 0, st, a, (int)p.grid);
 }
 
 }  // namespace
 
-#ifndef BIGMIN
-#define BIGMIN 1
-#endif
-#ifndef WHOLEMIN
-#define WHOLEMIN 1
-#endif
-#ifndef SPLITG
-#define SPLITG 2
-#endif
+// Which kernel, by the caller's largest row count (a hint: every kernel serves
+// every batch).  Measured on 256 CUs, us:
+// - up to 16 rows a sequence and KV head the decode kernel, whose waves share
+//   nothing but the rows; more rows would read the pages once per 16 of them.
+// - tiles of 64 rows, and of 256 (128 at head dim 128 in fp32 and at 256 in
+//   f16; at 256 in fp32 the registers leave no larger one) where there is one
+//   for every CU: 2048 rows of 32 / 4 heads of 128 over 8192 keys 272 against
+//   351.  At head dim 64, where staging is a smaller part, from two a CU on: five
+//   prompts of 777 46 against 48, one of 8000 (1000 tiles) 595 against 719.  At
+//   256, whose small tiles leave one wave a SIMD, from one for two CUs: 1500 rows
+//   over 3000 keys 116 against 143.
+// - tiles whole, one a block, where there is one for every CU (four prompts of
+//   300: 15 against 31 split); else equal stretches of their units for two
+//   blocks a CU (one at head dim 256, whose operands fill the LDS), and the
+//   join's launch: 300 rows over 5000 keys 62 against 90 whole.
 Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, int cus) {
     Kv4AttnPlan p = {};
-    const int group = n_head / n_kv, big = hd == 64 || (hd == 128 && f16) ? 256 : 128;
+    const int group = n_head / n_kv;
+    const int big = hd == 64 || (hd == 128 && f16) ? 256 : hd == 256 && !f16 ? 64 : 128;
     const long rows = (long)max_q * group;
     auto tiles = [&](int r) { return (long)n_tok * group / r * n_kv; };
-    p.rows = rows <= 16 ? 16 : rows > 64 && tiles(big) >= BIGMIN * cus ? big : 64;
-    p.whole = rows > 16 && (p.rows == big || tiles(p.rows) >= WHOLEMIN * cus);
-    p.grid = p.whole ? ((long)n_tok * group / p.rows + n_seq) * n_kv : (p.rows == 16 ? (hd != 256 ? 2 : 1) : hd != 256 ? SPLITG : 1) * cus;
-    p.chunk = p.rows == 16 ? 4 : 2;
+    p.rows = rows <= 16 ? 16 : rows > 64 && 2 * tiles(big) >= (hd == 64 ? 4 : hd == 128 ? 2 : 1) * cus ? big : 64;
+    p.whole = rows > 16 && (p.rows > 64 || tiles(p.rows) >= cus);
+    p.grid = p.whole ? ((long)n_tok * group / p.rows + n_seq) * n_kv : (hd != 256 ? 2 : 1) * cus;
+    p.chunk = p.rows == 16 ? 4 : 2;  // (a unit for each of the decode kernel's waves)
     p.part_bytes = p.whole ? 0 : (size_t)p.grid * 2 * p.rows * (hd + 4) * sizeof(float);
     p.work = p.whole ? 0 : KV4_COUNT_BYTES + p.part_bytes;
     return p;
