@@ -55,12 +55,14 @@ int cus_of(int device) {
     if (!n[device]) {
         int v = 0;
         if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || v < 1) v = 256;
-        if (v > KV4_MAX_BLOCKS / 4) v = KV4_MAX_BLOCKS / 4;
+        if (v > KV4_MAX_BLOCKS / 2) v = KV4_MAX_BLOCKS / 2;
         n[device] = v;
     }
     return n[device];
 }
 
+// Slots are ints, and a step of keys behind the last slot still is one.
+constexpr long MAX_SLOTS = 0x7FFFFF00L;
 bool page_size_ok(int ps) { return ps >= 16 && ps <= 256 && (ps & (ps - 1)) == 0; }
 bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -69,7 +71,7 @@ int view_of(const DracoKv4* c, Kv4View* v, const char* who) {
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return fail(-1, "%s: head dim %d not in {64, 128, 256}", who, c->head_dim);
     if (!page_size_ok(c->page_size)) return fail(-1, "%s: page size %d is no power of two in 16 .. 256", who, c->page_size);
-    if (c->n_kv < 1 || c->n_kv > 4096 || c->n_pages < 1 || (long)c->n_pages * c->page_size > 0x7FFFFFFFL)
+    if (c->n_kv < 1 || c->n_kv > 4096 || c->n_pages < 1 || (long)c->n_pages * c->page_size > MAX_SLOTS)
         return fail(-1, "%s: bad cache: %d KV heads, %d pages of %d", who, c->n_kv, c->n_pages, c->page_size);
     if (!aligned(c->data, 16)) return fail(-1, "%s: the pages are not 16-byte aligned", who);
     v->data = (uint8_t*)c->data;
@@ -105,8 +107,8 @@ int heads_ok(int n_head, int n_kv, const char* who) {
 int batch_ok(int n_seq, int max_blocks, int n_pages, int page_size, const char* who) {
     if (n_seq < 0 || max_blocks < 1 || n_pages < 1) return fail(-1, "%s: bad batch: %d sequences, %d blocks, %d pages", who, n_seq, max_blocks, n_pages);
     if (!page_size_ok(page_size)) return fail(-1, "%s: page size %d is no power of two in 16 .. 256", who, page_size);
-    if ((long)n_pages * page_size > 0x7FFFFFFFL || (long)max_blocks * page_size > 0x7FFFFFFFL)
-        return fail(-1, "%s: more than 2^31 - 1 slots", who);
+    if ((long)n_pages * page_size > MAX_SLOTS || (long)max_blocks * page_size > MAX_SLOTS)
+        return fail(-1, "%s: more than 2^31 - 256 slots", who);
     return 0;
 }
 
@@ -123,7 +125,7 @@ int attn_args(const DracoKv4* cache, const DracoKv4Attn* p, Kv4AttnArgs* a, bool
     if (int rc = type_of(p->code, f16, who)) return rc;
     if (int rc = heads_ok(p->n_head, cache->n_kv, who)) return rc;
     if (int rc = batch_ok(p->n_seq, p->max_blocks, cache->n_pages, cache->page_size, who)) return rc;
-    if (p->n_tok < 0 || (long)p->n_tok * p->n_head > 0x7FFFFFFFL) return fail(-1, "%s: n_tok %d", who, p->n_tok);
+    if (p->n_tok < 0 || (long)p->n_tok * p->n_head > MAX_SLOTS) return fail(-1, "%s: n_tok %d", who, p->n_tok);
     if (p->n_tok > 0 && p->n_seq > 0 && (p->max_q < 1 || p->max_len < 0))
         return fail(-1, "%s: max_q %d, max_len %d", who, p->max_q, p->max_len);
     if (p->window < 0 || p->sink < 0) return fail(-1, "%s: window %d, sink %d", who, p->window, p->sink);
@@ -149,7 +151,7 @@ int draco_kv_plan(const DracoKvPlan* p, void* stream) {
     const char* who = "draco_kv_plan";
     if (!p) return fail(-1, "%s: no arguments", who);
     if (int rc = batch_ok(p->n_seq, p->max_blocks, p->n_pages, p->page_size, who)) return rc;
-    if (p->n_tok < 0) return fail(-1, "%s: n_tok %d", who, p->n_tok);
+    if (p->n_tok < 0 || p->n_tok > 1 << 30) return fail(-1, "%s: n_tok %d", who, p->n_tok);
     if ((p->n_seq > 0 && (!p->block_table || !p->kv_len || !p->q_len || !p->kv_len_out)) || !p->free_list || !p->n_free ||
         !p->cu_q || (p->n_tok > 0 && !p->slot) || !p->n_free_out || !p->status || !p->work)
         return fail(-1, "%s: null pointer", who);
@@ -256,10 +258,10 @@ size_t draco_kv4_attn_workspace(const DracoKv4* cache, const DracoKv4Attn* p) {
     std::lock_guard<std::recursive_mutex> g(api_mutex());
     Kv4AttnArgs a = {};
     bool f16 = false;
-    if (attn_args(cache, p, &a, &f16) || p->n_tok == 0 || p->n_seq == 0) return 0;
+    if (attn_args(cache, p, &a, &f16)) return 0;
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) dev = 0;
-    return plan_of(cache, p, f16, cus_of(dev)).work;
+    return kv4_attn_workspace(cache->head_dim, cus_of(dev));
 }
 
 int draco_kv4_attn(const DracoKv4* cache, const DracoKv4Attn* p, void* stream) {

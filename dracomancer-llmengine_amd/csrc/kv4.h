@@ -26,7 +26,7 @@ namespace draco {
 struct Kv4View {
     uint8_t* data;
     unsigned page_bytes;  // n_kv * head_bytes (4096 heads of 256 tokens of 256 dims: 302 MB at most)
-    int head_bytes;   // ps * (hd + hd / 8)
+    int head_bytes;       // ps * (hd + hd / 8)
     int n_pages, ps_shift, n_kv, hd;
 };
 
@@ -68,13 +68,14 @@ struct Kv4AttnArgs {
 constexpr int KV4_MAX_BLOCKS = 4096;
 constexpr size_t KV4_COUNT_BYTES = KV4_MAX_BLOCKS * sizeof(int);
 struct Kv4AttnPlan {
-    int rows;            // of a tile: 16 (decode), else the chunk kernel's
+    int rows;            // of a tile: 16 and 32 the decode kernel's, else the prompt kernel's
     bool whole;
     long grid;
     int chunk;
     size_t part_bytes, work;  // bytes of partial rows, of workspace
 };
 Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, int cus);
+size_t kv4_attn_workspace(int hd, int cus);  // enough for any of its plans
 int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, void* work, hipStream_t st);
 
 struct KvPlanArgs {

@@ -17,6 +17,7 @@
 // each, and every product runs twice into one fp32 sum.  f16 rows: q is exact
 // and p is rounded once, to nearest (2^-12 of itself, as the output's own
 // rounding).
+#include <float.h>
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -436,7 +437,8 @@ __device__ __forceinline__ bool grows(const Row& w, float top) { return top > w.
 template <int MT>
 __device__ __forceinline__ float follow(Row& w, float top, f4v* acc) {  // what acc was multiplied by
     const bool grow = grows(w, top);
-    const float nfm = grow ? PBIAS - w.f * top : w.nfm;
+    // (a score past fp32's range gives p = inf and so NaN; with -inf here it would give 0)
+    const float nfm = grow ? fmaxf(PBIAS - w.f * top, -FLT_MAX) : w.nfm;
     const float keep = !grow ? 1.0f : w.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(nfm - w.nfm);
     if (grow) w.m = top;
     w.nfm = nfm;
@@ -637,8 +639,8 @@ __device__ __forceinline__ void join_waves(f4v* acc, float nfm, float& l, float*
     }
 }
 
-// Up to 16 rows of a sequence and KV head (decode): a block's waves take the
-// units of its piece in turn.  A wave's K words are free once the scores
+// Up to 16 NT rows of a sequence and KV head (decode, a few drafts): a block's
+// waves take the units of its piece in turn.  A wave's K words are free once the scores
 // are done and its V words once the output is: the loads of the unit DEPTH
 // turns later go there and then.  V scales (a lane's operands need all 16 of
 // its tokens', the same for 16 lanes) come as one 64th a lane and pass through
@@ -651,15 +653,15 @@ struct Raw {
     uint32_t vs[HD / 64];
     bool v_ok;
 };
-template <int HD, bool F16, int W, int DEPTH>
+template <int HD, bool F16, int W, int DEPTH, int NT>
 __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
-    constexpr int KS = HD / 32, MT = HD / 16, SROW = HD + 16;
+    constexpr int KS = HD / 32, MT = HD / 16, SROW = HD + 16, R = 16 * NT;
     __shared__ __align__(16) float smem[32 * W + W * MT * 64 * 4];
     __shared__ __align__(16) uint8_t s_vs[W][4 * SROW];
     const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     Work work;
     Batch batch;
-    if (!work_of<16>(a, work, batch, blockIdx.x, gridDim.x)) return;
+    if (!work_of<R>(a, work, batch, blockIdx.x, gridDim.x)) return;
     const int ps = 1 << a.c.ps_shift;
     Tile t;
     Units u;
@@ -697,15 +699,17 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
             w.vs[0] = x.x, w.vs[1] = x.y, w.vs[2] = x.z, w.vs[3] = x.w;
         }
     };
-    h8v qh[KS], ql[F16 ? 1 : KS];
-    float f;
+    h8v qh[NT][KS], ql[NT][F16 ? 1 : KS];
+    float f[NT];
     // the next piece, its q rows and its first units' loads
     auto begin = [&]() {
-        piece_of<16>(a, work, batch, t, u, part);
+        piece_of<R>(a, work, batch, t, u, part);
         const int n0 = part.lo + wave;
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) pages(n0 + W * d, kp[d], vp[d]);
-        load_q<HD, F16>(a, t, min(t.r0 + i, t.r1 - 1), qh, ql, f);  // rows past the last repeat it
+#pragma unroll
+        for (int x = 0; x < NT; x++)  // (rows past the last repeat it)
+            load_q<HD, F16>(a, t, min(t.r0 + 16 * x + i, t.r1 - 1), qh[x], ql[x], f[x]);
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) {
             load_k(n0 + W * d, kp[d], raw[d]);
@@ -716,41 +720,50 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
     Shares shares;
     begin();
     for (;;) {
-        Row w;
-        row_init(a, t, min(t.r0 + i, t.r1 - 1), f, w);
-        const Whole whole = whole_of(a, t, t.r0, t.r1);
-        f4v acc[MT];
+        Row w[NT];
+        f4v acc[NT][MT];
 #pragma unroll
-        for (int m = 0; m < MT; m++) acc[m] = f4v{0, 0, 0, 0};
+        for (int x = 0; x < NT; x++) {
+            row_init(a, t, min(t.r0 + 16 * x + i, t.r1 - 1), f[x], w[x]);
+#pragma unroll
+            for (int m = 0; m < MT; m++) acc[x][m] = f4v{0, 0, 0, 0};
+        }
+        const Whole whole = whole_of(a, t, t.r0, t.r1);
         for (int base = part.lo + wave; base < part.hi; base += W * DEPTH) {
 #pragma unroll
             for (int d = 0; d < DEPTH; d++) {
                 const int n = base + W * d;
                 if (n >= part.hi) break;
-                Raw<HD>& x = raw[d];
+                Raw<HD>& z = raw[d];
                 const int key0 = u.at(n) * UNIT, next = n + W * DEPTH;
-                f4v c[4];
+                f4v c[NT][4];
 #pragma unroll
-                for (int y = 0; y < 4; y++) c[y] = f4v{0, 0, 0, 0};
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) c[x][y] = f4v{0, 0, 0, 0};
 #pragma unroll
                 for (int s = 0; s < KS; s++)
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
-                        const h8v o = k_operand(x.k[y].w[s], x.k[y].scale(s));
-                        c[y] = mfma(o, qh[s], c[y]);
-                        if constexpr (!F16) c[y] = mfma(o, ql[s], c[y]);
+                        const h8v o = k_operand(z.k[y].w[s], z.k[y].scale(s));
+#pragma unroll
+                        for (int x = 0; x < NT; x++) {
+                            c[x][y] = mfma(o, qh[x][s], c[x][y]);
+                            if constexpr (!F16) c[x][y] = mfma(o, ql[x][s], c[x][y]);
+                        }
                     }
                 const int vnext = vp[0];
-                load_k(next, kp[0], x);
+                load_k(next, kp[0], z);
                 pages(next + W, kp[0], vp[0]);
-                h8v ph[2], pl[2];
-                softmax<F16, MT>(w, whole.has(key0), key0, a.sink, c, acc, ph, pl);
+                h8v ph[NT][2], pl[NT][2];
+#pragma unroll
+                for (int x = 0; x < NT; x++) softmax<F16, MT>(w[x], whole.has(key0), key0, a.sink, c[x], acc[x], ph[x], pl[x]);
                 // scales of this lane: tokens 16 g + HD / 32 * (i % (512 / HD)) .. of block i / (512 / HD)
                 uint32_t vs[HD / 64];
 #pragma unroll
-                for (int y = 0; y < HD / 64; y++) vs[y] = x.vs[y];
-                if (key0 + UNIT > t.len || !x.v_ok) {
-                    const int key = key0 + 16 * g + (HD / 32) * (i % (512 / HD)), len = x.v_ok ? t.len : 0;
+                for (int y = 0; y < HD / 64; y++) vs[y] = z.vs[y];
+                if (key0 + UNIT > t.len || !z.v_ok) {
+                    const int key = key0 + 16 * g + (HD / 32) * (i % (512 / HD)), len = z.v_ok ? t.len : 0;
 #pragma unroll
                     for (int y = 0; y < HD / 64; y++)
                         vs[y] = key + 2 * y + 1 < len ? vs[y] : key + 2 * y < len ? vs[y] & 0xFFFFu : 0;
@@ -764,18 +777,21 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
 #pragma unroll
                     for (int y = 0; y < 2; y++) {
                         VPart v;
-                        v.w = y ? u2v{x.v[b].z, x.v[b].w} : u2v{x.v[b].x, x.v[b].y};
+                        v.w = y ? u2v{z.v[b].z, z.v[b].w} : u2v{z.v[b].x, z.v[b].y};
                         v.s = *(const u4v*)(sv + g * SROW + b * 32 + y * 16);
                         h8v lo, hi;
                         v_operands(v, lo, hi);
-                        acc[2 * b] = mfma(lo, ph[y], acc[2 * b]);
-                        acc[2 * b + 1] = mfma(hi, ph[y], acc[2 * b + 1]);
-                        if constexpr (!F16) {
-                            acc[2 * b] = mfma(lo, pl[y], acc[2 * b]);
-                            acc[2 * b + 1] = mfma(hi, pl[y], acc[2 * b + 1]);
+#pragma unroll
+                        for (int x = 0; x < NT; x++) {
+                            acc[x][2 * b] = mfma(lo, ph[x][y], acc[x][2 * b]);
+                            acc[x][2 * b + 1] = mfma(hi, ph[x][y], acc[x][2 * b + 1]);
+                            if constexpr (!F16) {
+                                acc[x][2 * b] = mfma(lo, pl[x][y], acc[x][2 * b]);
+                                acc[x][2 * b + 1] = mfma(hi, pl[x][y], acc[x][2 * b + 1]);
+                            }
                         }
                     }
-                load_v(next, vnext, x);
+                load_v(next, vnext, z);
             }
         }
         // the next piece's loads are on their way while this one is put together
@@ -783,18 +799,21 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
         const Shared sh = shared_of(work, part);
         const bool more = work.left > 0;
         if (more) begin();
-        float l = w.l, nfm;
-        f4v o[tiles_of_wave(HD, W)];
-        join_waves<HD, W>(acc, w.nfm, l, &nfm, smem, o);
-        if (done.r0 + i < done.r1 && wave < MT) {
+#pragma unroll
+        for (int x = 0; x < NT; x++) {
+            float l = w[x].l, nfm;
+            f4v o[tiles_of_wave(HD, W)];
+            join_waves<HD, W>(acc[x], w[x].nfm, l, &nfm, smem, o);
+            const int r = done.r0 + 16 * x + i;
+            if (r >= done.r1 || wave >= MT) continue;
             if (!sh.split()) {
                 const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-                const long at = out_at(a, done, done.r0 + i, HD);
+                const long at = out_at(a, done, r, HD);
 #pragma unroll
                 for (int c = 0; c < tiles_of_wave(HD, W); c++) store4<F16>(a, at + 16 * (c * W + wave) + 4 * g, o[c] * inv);
             } else {
                 const Parts parts = parts_of(a);
-                const unsigned row = part_at<HD, 16>(sh.slot(blockIdx.x), i);
+                const unsigned row = part_at<HD, R>(sh.slot(blockIdx.x), r - done.r0);
 #pragma unroll
                 for (int c = 0; c < tiles_of_wave(HD, W); c++) parts.put4(row + 16 * (c * W + wave) + 4 * g, o[c]);
                 if (wave == 0 && g == 0) parts.put4(row + HD, f4v{l, nfm, 0, 0});
@@ -803,7 +822,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
         if (sh.split()) shares.add(sh, done);
         if (!more) break;
     }
-    join_blocks<HD, F16, 16, 64 * W>(a, shares);
+    join_blocks<HD, F16, R, 64 * W>(a, shares);
 }
 
 // More rows (drafts, prompts): W waves of 16 NT rows over the same units, whose
@@ -1132,7 +1151,9 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid);
     constexpr int NT = HD == 64 || (HD == 128 && F16) ? 2 : 1;  // row tiles a wave of the large tiles
     if (p.rows == 16) {
-        hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, HD == 256 ? 2 : 1>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, HD == 256 ? 2 : 1, 1>), grid, dim3(256), 0, st, a);
+    } else if (HD == 128 && p.rows == 32) {
+        hipLaunchKernelGGL((k_kv4_attn<128, F16, 4, 1, 2>), grid, dim3(256), 0, st, a);
     } else if (p.rows == 64) {
         hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 4, 1, true>), grid, dim3(256), 0, st, a);
         if (p.whole) return;
@@ -1149,6 +1170,11 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
 // every batch).  Measured on 256 CUs, us:
 // - up to 16 rows a sequence and KV head the decode kernel, whose waves share
 //   nothing but the rows; more rows would read the pages once per 16 of them.
+// - up to 32 at head dim 128 the same with two row tiles (356 registers, so one
+//   block a CU): 24 sequences of 5 drafts over 20011 keys, window 6001, 32 / 8
+//   heads, in fp32 75 against 116 in tiles of 64, 8 of 16 in f16 51 against 54.
+//   At 64 (12 drafts of 32 / 8 heads over 8000 keys 73 against 55) and at 256,
+//   where they spill (5 drafts 98 against 71), the tiles of 64 are faster.
 // - tiles of 64 rows, and of 256 (128 at head dim 128 in fp32 and at 256 in
 //   f16; at 256 in fp32 the registers leave no larger one) where there is one
 //   for every CU: 2048 rows of 32 / 4 heads of 128 over 8192 keys 272 against
@@ -1167,12 +1193,18 @@ Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, in
     const long rows = (long)max_q * group;
     auto tiles = [&](int r) { return (long)n_tok * group / r * n_kv; };
     p.rows = rows <= 16 ? 16 : rows > 64 && 2 * tiles(big) >= (hd == 64 ? 4 : hd == 128 ? 2 : 1) * cus ? big : 64;
-    p.whole = rows > 16 && (p.rows > 64 || tiles(p.rows) >= cus);
-    p.grid = p.whole ? ((long)n_tok * group / p.rows + n_seq) * n_kv : (hd != 256 ? 2 : 1) * cus;
-    p.chunk = p.rows == 16 ? 4 : 2;  // (a unit for each of the decode kernel's waves)
+    if (hd == 128 && p.rows == 64 && rows <= 32) p.rows = 32;
+    p.whole = p.rows > 64 || (p.rows == 64 && tiles(64) >= cus);
+    p.grid = p.whole ? ((long)n_tok * group / p.rows + n_seq) * n_kv : (p.rows != 32 && hd != 256 ? 2 : 1) * cus;
+    p.chunk = p.rows <= 32 ? 4 : 2;  // (a unit for each of the decode kernel's waves)
     p.part_bytes = p.whole ? 0 : (size_t)p.grid * 2 * p.rows * (hd + 4) * sizeof(float);
     p.work = p.whole ? 0 : KV4_COUNT_BYTES + p.part_bytes;
     return p;
+}
+
+// Of split tiles of 64 rows, the most of any plan.
+size_t kv4_attn_workspace(int hd, int cus) {
+    return KV4_COUNT_BYTES + (size_t)(hd != 256 ? 2 : 1) * cus * 2 * 64 * (hd + 4) * sizeof(float);
 }
 
 int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, void* work, hipStream_t st) {

@@ -510,9 +510,10 @@ size_t draco_kv4_page_bytes(int page_size, int n_kv, int head_dim);
  * whose pages are not all there (ascending order decides), or that would pass
  * max_blocks pages or n_tok rows, is refused: its rows get position and slot
  * -1, its length and pages stay, later ones are still served where they need
- * no page or enough are left of the count before the refused.  status[0] =
+ * no page or enough are left of the count before the refused.  (Its rows stay
+ * in cu_q; what attention gives for them means nothing.)  status[0] =
  * sequences refused, status[1] = rows beyond n_tok.  Negative lengths count
- * as 0.  `work`: one int, 0 before its first use and left 0; calls that
+ * as 0.  A page belongs to one sequence.  `work`: one int, 0 before its first use and left 0; calls that
  * overlap need their own. */
 typedef struct {
     int n_seq, max_blocks, n_pages, page_size, n_tok;
@@ -564,8 +565,9 @@ int draco_kv_release(const DracoKvRelease* p, void* stream);
  * turns by row pos[axis[i]][token] of `table` ([table_rows][rot/2] of cos,
  * sin: draco_rope_table's layout).  Text has one axis; images and video up to
  * four (time, height, width, ...), each with its own positions, pos_stride
- * ints apart.  Products and sums in 64 bits, one rounding to fp32 (f16 q: another to f16).  A position outside
- * the table makes its pairs NaN.  q_out may be q with pairing 0 or rot 0 only.
+ * ints apart.  Products and sums in 64 bits, one rounding to fp32 (f16 q:
+ * another to f16).  A position outside the table makes its pairs NaN.  q_out
+ * may be q with pairing 0 or rot 0 only, and overlaps no input otherwise.
  *
  * A k or v row that is not finite is held as NaN: attention rows that see the
  * token become NaN, others do not.  Magnitudes past 65472 saturate. */
@@ -601,14 +603,16 @@ int draco_kv4_read(const DracoKv4* cache, const int* slot, int n, float* k, floa
  * draco_kv4_append (out must not be q).  One call serves decode (one row a
  * sequence), drafts and prompt chunks, mixed as they come.
  *
- * max_q, max_len: the largest row count and length of a sequence, or more;
- * smaller values only cost speed.  A length past max_blocks pages, or a page
- * outside the pool that a row sees, gives NaN.  work / work_bytes: at least
- * draco_kv4_attn_workspace(cache, p) bytes (it reads sizes only), 16-byte
- * aligned.  Its first 16 KiB (counters) are 0 before its first use; calls of
- * any shapes leave them 0 again, so one allocation of the largest size serves
- * them all.  Calls that overlap need their own.  A call's results are the same
- * every time. */
+ * max_q: the largest row count of a sequence, or more; a smaller value only
+ * costs speed.  max_len: the largest length, or more (0 or more; nothing
+ * depends on it now).  A length past max_blocks pages, a page outside the pool
+ * that a row sees, or a score past fp32's range gives NaN.
+ *
+ * work / work_bytes: draco_kv4_attn_workspace(cache, p) bytes, 16-byte
+ * aligned, which depend on head_dim and the current device only: one
+ * allocation serves calls of every batch and shape, one at a time (calls that
+ * overlap need their own).  Its first 16 KiB (counters) are 0 before its first
+ * use and left 0.  A call's results are the same every time. */
 typedef struct {
     int code;
     int n_seq, n_tok, max_q, max_len;

@@ -412,6 +412,101 @@ def test_attn_long_splits(dev, hd, code, window, sink):
     assert out.shape[0] == 7
 
 
+def check_sampled(c, lens, qlens, nh, rng, code, window, sink, n_sample):
+    """check_attn at n_sample of the rows, the first and last of the longest sequence among them."""
+    held = fill(c, lens, rng, code)
+    cu = np.concatenate([[0], np.cumsum(qlens)])
+    q = (1.5 * rng.standard_normal((int(cu[-1]), nh, c.hd))).astype(NP[code])
+    out = c.attn(q, cu, lens, code=code, window=window, sink=sink)
+    big = int(np.argmax(qlens))
+    rows = np.unique(np.concatenate([[cu[big], cu[big + 1] - 1], rng.choice(int(cu[-1]), min(n_sample, int(cu[-1])), replace=False)]))
+    for r in rows:
+        s = int(np.searchsorted(cu, r, "right") - 1)
+        n, (k, v) = lens[s], held[s]
+        want, top = R.attention(q[r:r + 1], k, v, np.array([n - (cu[s + 1] - r)]), c.hd ** -0.5, window, sink)
+        err = float(np.abs(out[r:r + 1].astype(np.float64) - want).max())
+        lim = bound(code, c.hd, n, top, float(np.abs(v).max()))
+        assert np.isfinite(out[r].astype(np.float64)).all() and err <= lim, (s, r, err, lim)
+    assert np.isfinite(out.astype(np.float64)).all()
+
+
+# Row counts at which an MI355X has tiles for every CU: of 256 rows at head dims
+# 64 and 128 (f16), of 128 at 128 (fp32) and 256 (f16), of 64 below those.
+@pytest.mark.parametrize("hd,nh,nkv,code", [(128, 60, 4, F16), (128, 32, 4, F32), (64, 128, 8, F32), (64, 128, 8, F16), (256, 16, 2, F16),
+                                            (256, 16, 2, F32), (128, 16, 4, F32), (128, 20, 4, F16), (64, 32, 4, F16)])
+@pytest.mark.parametrize("window,sink", [(0, 0), (150, 70)])
+def test_attn_tiles_for_every_cu(dev, hd, nh, nkv, code, window, sink):
+    rng = np.random.default_rng(hd + nh + window)
+    lens, qlens = [901, 257, 0, 90], [790, 257, 0, 61]
+    check_sampled(Cache(dev, lens, nkv, hd, 32), lens, qlens, nh, rng, code, window, sink, 24)
+
+
+@pytest.mark.parametrize("hd,nh,nkv,code", [(64, 4, 2, F32), (128, 8, 2, F32), (128, 4, 1, F16), (256, 4, 2, F16)])
+@pytest.mark.parametrize("most", [1, 4, 7, 30])
+def test_attn_many_sequences(dev, hd, nh, nkv, code, most):
+    """More sequences than a wave reads at once, some without rows or keys: decode, drafts and chunks."""
+    rng = np.random.default_rng(hd + most)
+    qlens = [int(x) for x in rng.integers(0, most + 1, 150)]
+    qlens[70] = most
+    lens = [int(m + x * (rng.random() < 0.7)) for m, x in zip(qlens, rng.integers(0, 300, 150))]
+    check_sampled(Cache(dev, lens, nkv, hd, 16), lens, qlens, nh, rng, code, 40 if most == 4 else 0, 3, 60)
+
+
+@pytest.mark.parametrize("hd,code", [(64, F32), (128, F16)])
+@pytest.mark.parametrize("n_seq", [300, 4500])
+def test_attn_whole_tiles_of_many_sequences(dev, hd, code, n_seq):
+    """The search for a block's sequence in one, two and three steps of 64."""
+    rng = np.random.default_rng(hd + n_seq)
+    qlens = [int(x) for x in rng.integers(0, 8, n_seq)]
+    qlens[n_seq // 2] = 30
+    lens = [m + int(x) for m, x in zip(qlens, rng.integers(0, 12, n_seq))]
+    check_sampled(Cache(dev, lens, 1, hd, 16), lens, qlens, 16, rng, code, 0, 0, 80)
+
+
+@pytest.mark.parametrize("hd,code", [(64, F32), (128, F32), (128, F16), (256, F32), (256, F16)])
+def test_one_workspace_for_every_shape(dev, hd, code):
+    """Calls of different kinds one after another over one workspace, nothing cleared between them."""
+    rng = np.random.default_rng(hd)
+    lens = [700, 90, 333]
+    c = Cache(dev, lens, 2, hd, 16)
+    held = fill(c, lens, rng, code)
+    work = None
+    for qlens in ([1, 1, 1], [5, 3, 0], [6, 7, 7], [20, 1, 31], [300, 90, 200], [1, 0, 1], [16, 2, 9], [6, 7, 7]):
+        cu = np.concatenate([[0], np.cumsum(qlens)])
+        q = (1.5 * rng.standard_normal((int(cu[-1]), 8, hd))).astype(NP[code])
+        out = dev.up(np.full(q.shape, -777.0, NP[code]))
+        a = c.attn_args(q, out, cu, lens, code=code)
+        if work is None:
+            work = a.work, a.work_bytes
+        a.work, a.work_bytes = work
+        c.lib.check(c.L.draco_kv4_attn(ct.byref(c.desc), ct.byref(a), None), "draco_kv4_attn")
+        got = dev.down(out, q.shape, NP[code]).astype(np.float64)
+        for s in range(3):
+            rows = np.unique(np.clip([0, 1, 5, qlens[s] // 2, qlens[s] - 1], 0, max(qlens[s] - 1, 0)))[:qlens[s]]
+            if not len(rows):
+                continue
+            k, v = held[s]
+            want, big = R.attention(q[cu[s] + rows], k, v, lens[s] - qlens[s] + rows, hd ** -0.5, 0, 0)
+            err = float(np.abs(got[cu[s] + rows] - want).max())
+            assert err <= bound(code, hd, lens[s], big, float(np.abs(v).max())), (qlens, s, err)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("m", [1, 7, 90])
+def test_attn_scores_past_fp32_are_nan(dev, hd, m):
+    """A row whose scores pass fp32's range is NaN (never a silent 0); the rows beside it are not touched."""
+    rng = np.random.default_rng(hd + m)
+    n = 200
+    c = Cache(dev, [n], 1, hd, 16)
+    k, v = np.ones((n, 1, hd), np.float32), rng.standard_normal((n, 1, hd)).astype(np.float32)
+    c.append(None, k, v, c.slots(0, 0, n))
+    q = rng.standard_normal((m, 4, hd)).astype(np.float32)
+    q[:, 1] = 3e37
+    q[:, 2] = -3e37
+    out = c.attn(q, [0, m], [n], scale=8.0)
+    assert np.isnan(out[:, 1:3]).all() and np.isfinite(out[:, [0, 3]]).all()
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("m", [1, 40, 200])
 def test_attn_nan_stays_with_the_rows_that_see_it(dev, hd, m):

@@ -102,3 +102,28 @@ def test_nothing_to_do_is_no_error():
     assert L.draco_kv4_append(ct.byref(c), ct.byref(append(n_tok=0)), None) == 0
     assert L.draco_kv4_read(ct.byref(c), P, 0, P, P, None) == 0
     assert L.draco_kv4_attn(ct.byref(c), ct.byref(attn(n_tok=0, n_seq=0)), None) == 0
+
+
+@pytest.mark.parametrize("n,ok", [((0x7FFFFF00 // 16), True), ((0x7FFFFF00 // 16) + 1, False)])
+def test_slots_stay_ints_a_step_past_the_last(n, ok):
+    """2^31 - 256 slots at most: the last step of keys of a sequence may begin in them and end behind them."""
+    c = cache(n_pages=n)
+    rc = L.draco_kv4_read(ct.byref(c), P, 0, P, P, None)
+    assert rc == (0 if ok else -1)
+    rc = L.draco_kv4_attn(ct.byref(cache()), ct.byref(attn(max_blocks=n, n_tok=0)), None)
+    assert rc == (0 if ok else -1)
+    if not ok:
+        assert "slots" in lib.last_error()
+
+
+def test_more_rows_than_ints_count():
+    refused(L.draco_kv_plan(ct.byref(lib.KvPlan(n_seq=0, max_blocks=1, n_pages=1, page_size=16, n_tok=(1 << 30) + 1)), None), "n_tok")
+    refused(L.draco_kv4_attn(ct.byref(cache()), ct.byref(attn(n_tok=0x7FFFFFFF // 4)), None), "n_tok")
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_one_workspace_size_serves_every_batch(hd):
+    c = cache(head_dim=hd)
+    sizes = {L.draco_kv4_attn_workspace(ct.byref(c), ct.byref(attn(code=code, n_seq=s, n_tok=t, max_q=q, n_head=h)))
+             for code in (7, 9) for s, t, q in ((0, 0, 1), (1, 1, 1), (3, 70, 50), (9, 4000, 4000)) for h in (2, 64)}
+    assert len(sizes) == 1 and sizes.pop() >= 16384
