@@ -134,7 +134,10 @@ int attn_args(const DracoKv4* cache, const DracoKv4Attn* p, Kv4AttnArgs* a, bool
 }
 
 Kv4AttnPlan plan_of(const DracoKv4* c, const DracoKv4Attn* p, bool f16, int cus) {
-    return kv4_attn_plan(c->head_dim, f16, p->n_seq, p->n_tok, p->n_head, c->n_kv, p->max_q < p->n_tok ? p->max_q : p->n_tok, cus);
+    const int max_q = p->max_q < p->n_tok ? p->max_q : p->n_tok;
+    long keys = p->max_len;  // that a row sees, at most
+    if (p->window > 0 && (long)p->window + p->sink < keys) keys = (long)p->window + p->sink;
+    return kv4_attn_plan(c->head_dim, f16, p->n_seq, p->n_tok, p->n_head, c->n_kv, max_q, keys, cus);
 }
 
 }  // namespace

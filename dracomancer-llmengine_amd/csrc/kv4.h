@@ -74,7 +74,8 @@ struct Kv4AttnPlan {
     int chunk;
     size_t part_bytes, work;  // bytes of partial rows, of workspace
 };
-Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, int cus);
+Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, long max_keys,
+                          int cus);
 size_t kv4_attn_workspace(int hd, int cus);  // enough for any of its plans
 int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, void* work, hipStream_t st);
 

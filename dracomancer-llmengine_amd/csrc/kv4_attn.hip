@@ -502,6 +502,13 @@ __device__ __forceinline__ unsigned part_at(long slot, int row) {  // floats int
     return (unsigned)((slot * R + row) * (HD + 4));
 }
 
+// The tile that a block was the first on and left unfinished, for the join's
+// launch; no rows: none.
+struct alignas(16) Left {
+    int q0, head, r0, r1, b1, pad[3];
+};
+__device__ __forceinline__ Left* left_of(const Kv4AttnArgs& a, int block) { return (Left*)((char*)a.part + a.part_bytes) + block; }
+
 // Partial rows pass between blocks on different XCDs, whose L2s do not see each
 // other's lines.  They are written and read past the L2s (cache policy sc1, as
 // device-scope atomics are), and the writer waits for its stores before the
@@ -641,8 +648,8 @@ __device__ __forceinline__ void join_waves(f4v* acc, float nfm, float& l, float*
 
 // Up to 16 NT rows of a sequence and KV head (decode, a few drafts): a block's
 // waves take the units of its piece in turn.  A wave's K words are free once the scores
-// are done and its V words once the output is: the loads of the unit DEPTH
-// turns later go there and then.  V scales (a lane's operands need all 16 of
+// are done and its V words once the output is: the loads of the wave's next
+// unit go there and then.  V scales (a lane's operands need all 16 of
 // its tokens', the same for 16 lanes) come as one 64th a lane and pass through
 // LDS, which takes 8 wide loads and 32 registers less than loading them to
 // every lane.
@@ -653,7 +660,7 @@ struct Raw {
     uint32_t vs[HD / 64];
     bool v_ok;
 };
-template <int HD, bool F16, int W, int DEPTH, int NT>
+template <int HD, bool F16, int W, int NT>
 __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
     constexpr int KS = HD / 32, MT = HD / 16, SROW = HD + 16, R = 16 * NT;
     __shared__ __align__(16) float smem[32 * W + W * MT * 64 * 4];
@@ -666,8 +673,8 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
     Tile t;
     Units u;
     Piece part;
-    Raw<HD> raw[DEPTH];
-    int kp[DEPTH], vp[DEPTH];  // pages of the units to load next
+    Raw<HD> z;
+    int kp, vp;  // pages of the unit to load next
     // (Past the piece's end its last unit is loaded again: behind a branch the
     // compiler could not tell which loads are in flight and would wait for all.)
     auto unit_of = [&](int n) { return u.at(max(min(n, part.hi - 1), 0)); };
@@ -675,28 +682,28 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
         k = page_of(a, t.table, k_key(unit_of(n)));
         v = page_of(a, t.table, v_key(unit_of(n)));
     };
-    auto load_k = [&](int n, int page, Raw<HD>& w) {
+    auto load_k = [&](int n, int page) {
         bool ok;
         const int key = k_key(unit_of(n)), off = key & (ps - 1);
         const uint8_t* p = page_ptr(a, page, key, t.head, ok);
 #pragma unroll
-        for (int x = 0; x < 4; x++) load_krow<HD, KS>(p, ok, ps, off + 4 * x, 0, w.k[x]);
+        for (int x = 0; x < 4; x++) load_krow<HD, KS>(p, ok, ps, off + 4 * x, 0, z.k[x]);
     };
-    auto load_v = [&](int n, int page, Raw<HD>& w) {
+    auto load_v = [&](int n, int page) {
         const int key = v_key(unit_of(n)), grp = (key & (ps - 1)) >> 4;
-        const uint8_t* p = page_ptr(a, page, key, t.head, w.v_ok);
+        const uint8_t* p = page_ptr(a, page, key, t.head, z.v_ok);
         const uint8_t* c = p + ps * (HD / 2) + grp * (HD * 8) + i * 16;
 #pragma unroll
-        for (int b = 0; b < KS; b++) w.v[b] = *gptr<u4v>(c + b * 256);
+        for (int b = 0; b < KS; b++) z.v[b] = *gptr<u4v>(c + b * 256);
         const uint8_t* s = p + ps * HD + ps * (HD / 16) + grp * HD + i * (HD / 16);
         if constexpr (HD == 64) {
-            w.vs[0] = *gptr<uint32_t>(s);
+            z.vs[0] = *gptr<uint32_t>(s);
         } else if constexpr (HD == 128) {
             const u2v x = *gptr<u2v>(s);
-            w.vs[0] = x.x, w.vs[1] = x.y;
+            z.vs[0] = x.x, z.vs[1] = x.y;
         } else {
             const u4v x = *gptr<u4v>(s);
-            w.vs[0] = x.x, w.vs[1] = x.y, w.vs[2] = x.z, w.vs[3] = x.w;
+            z.vs[0] = x.x, z.vs[1] = x.y, z.vs[2] = x.z, z.vs[3] = x.w;
         }
     };
     h8v qh[NT][KS], ql[NT][F16 ? 1 : KS];
@@ -705,17 +712,13 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
     auto begin = [&]() {
         piece_of<R>(a, work, batch, t, u, part);
         const int n0 = part.lo + wave;
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++) pages(n0 + W * d, kp[d], vp[d]);
+        pages(n0, kp, vp);
 #pragma unroll
         for (int x = 0; x < NT; x++)  // (rows past the last repeat it)
             load_q<HD, F16>(a, t, min(t.r0 + 16 * x + i, t.r1 - 1), qh[x], ql[x], f[x]);
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++) {
-            load_k(n0 + W * d, kp[d], raw[d]);
-            load_v(n0 + W * d, vp[d], raw[d]);
-        }
-        pages(n0 + W * DEPTH, kp[0], vp[0]);
+        load_k(n0, kp);
+        load_v(n0, vp);
+        pages(n0 + W, kp, vp);
     };
     Shares shares;
     begin();
@@ -729,70 +732,64 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
             for (int m = 0; m < MT; m++) acc[x][m] = f4v{0, 0, 0, 0};
         }
         const Whole whole = whole_of(a, t, t.r0, t.r1);
-        for (int base = part.lo + wave; base < part.hi; base += W * DEPTH) {
+        for (int n = part.lo + wave; n < part.hi; n += W) {
+            const int key0 = u.at(n) * UNIT, next = n + W;
+            f4v c[NT][4];
 #pragma unroll
-            for (int d = 0; d < DEPTH; d++) {
-                const int n = base + W * d;
-                if (n >= part.hi) break;
-                Raw<HD>& z = raw[d];
-                const int key0 = u.at(n) * UNIT, next = n + W * DEPTH;
-                f4v c[NT][4];
+            for (int x = 0; x < NT; x++)
 #pragma unroll
-                for (int x = 0; x < NT; x++)
+                for (int y = 0; y < 4; y++) c[x][y] = f4v{0, 0, 0, 0};
 #pragma unroll
-                    for (int y = 0; y < 4; y++) c[x][y] = f4v{0, 0, 0, 0};
+            for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int s = 0; s < KS; s++)
+                for (int y = 0; y < 4; y++) {
+                    const h8v o = k_operand(z.k[y].w[s], z.k[y].scale(s));
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        const h8v o = k_operand(z.k[y].w[s], z.k[y].scale(s));
-#pragma unroll
-                        for (int x = 0; x < NT; x++) {
-                            c[x][y] = mfma(o, qh[x][s], c[x][y]);
-                            if constexpr (!F16) c[x][y] = mfma(o, ql[x][s], c[x][y]);
-                        }
+                    for (int x = 0; x < NT; x++) {
+                        c[x][y] = mfma(o, qh[x][s], c[x][y]);
+                        if constexpr (!F16) c[x][y] = mfma(o, ql[x][s], c[x][y]);
                     }
-                const int vnext = vp[0];
-                load_k(next, kp[0], z);
-                pages(next + W, kp[0], vp[0]);
-                h8v ph[NT][2], pl[NT][2];
-#pragma unroll
-                for (int x = 0; x < NT; x++) softmax<F16, MT>(w[x], whole.has(key0), key0, a.sink, c[x], acc[x], ph[x], pl[x]);
-                // scales of this lane: tokens 16 g + HD / 32 * (i % (512 / HD)) .. of block i / (512 / HD)
-                uint32_t vs[HD / 64];
-#pragma unroll
-                for (int y = 0; y < HD / 64; y++) vs[y] = z.vs[y];
-                if (key0 + UNIT > t.len || !z.v_ok) {
-                    const int key = key0 + 16 * g + (HD / 32) * (i % (512 / HD)), len = z.v_ok ? t.len : 0;
-#pragma unroll
-                    for (int y = 0; y < HD / 64; y++)
-                        vs[y] = key + 2 * y + 1 < len ? vs[y] : key + 2 * y < len ? vs[y] & 0xFFFFu : 0;
                 }
-                uint8_t* sv = s_vs[wave];
-                if constexpr (HD == 64) *(uint32_t*)(sv + g * SROW + i * 4) = vs[0];
-                else if constexpr (HD == 128) *(u2v*)(sv + g * SROW + i * 8) = u2v{vs[0], vs[1]};
-                else *(u4v*)(sv + g * SROW + i * 16) = u4v{vs[0], vs[1], vs[2], vs[3]};
+            const int vnext = vp;
+            load_k(next, kp);
+            pages(next + W, kp, vp);
+            h8v ph[NT][2], pl[NT][2];
 #pragma unroll
-                for (int b = 0; b < KS; b++)
+            for (int x = 0; x < NT; x++) softmax<F16, MT>(w[x], whole.has(key0), key0, a.sink, c[x], acc[x], ph[x], pl[x]);
+            // scales of this lane: tokens 16 g + HD / 32 * (i % (512 / HD)) .. of block i / (512 / HD)
+            uint32_t vs[HD / 64];
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        VPart v;
-                        v.w = y ? u2v{z.v[b].z, z.v[b].w} : u2v{z.v[b].x, z.v[b].y};
-                        v.s = *(const u4v*)(sv + g * SROW + b * 32 + y * 16);
-                        h8v lo, hi;
-                        v_operands(v, lo, hi);
+            for (int y = 0; y < HD / 64; y++) vs[y] = z.vs[y];
+            if (key0 + UNIT > t.len || !z.v_ok) {
+                const int key = key0 + 16 * g + (HD / 32) * (i % (512 / HD)), len = z.v_ok ? t.len : 0;
 #pragma unroll
-                        for (int x = 0; x < NT; x++) {
-                            acc[x][2 * b] = mfma(lo, ph[x][y], acc[x][2 * b]);
-                            acc[x][2 * b + 1] = mfma(hi, ph[x][y], acc[x][2 * b + 1]);
-                            if constexpr (!F16) {
-                                acc[x][2 * b] = mfma(lo, pl[x][y], acc[x][2 * b]);
-                                acc[x][2 * b + 1] = mfma(hi, pl[x][y], acc[x][2 * b + 1]);
-                            }
+                for (int y = 0; y < HD / 64; y++)
+                    vs[y] = key + 2 * y + 1 < len ? vs[y] : key + 2 * y < len ? vs[y] & 0xFFFFu : 0;
+            }
+            uint8_t* sv = s_vs[wave];
+            if constexpr (HD == 64) *(uint32_t*)(sv + g * SROW + i * 4) = vs[0];
+            else if constexpr (HD == 128) *(u2v*)(sv + g * SROW + i * 8) = u2v{vs[0], vs[1]};
+            else *(u4v*)(sv + g * SROW + i * 16) = u4v{vs[0], vs[1], vs[2], vs[3]};
+#pragma unroll
+            for (int b = 0; b < KS; b++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    VPart v;
+                    v.w = y ? u2v{z.v[b].z, z.v[b].w} : u2v{z.v[b].x, z.v[b].y};
+                    v.s = *(const u4v*)(sv + g * SROW + b * 32 + y * 16);
+                    h8v lo, hi;
+                    v_operands(v, lo, hi);
+#pragma unroll
+                    for (int x = 0; x < NT; x++) {
+                        acc[x][2 * b] = mfma(lo, ph[x][y], acc[x][2 * b]);
+                        acc[x][2 * b + 1] = mfma(hi, ph[x][y], acc[x][2 * b + 1]);
+                        if constexpr (!F16) {
+                            acc[x][2 * b] = mfma(lo, pl[x][y], acc[x][2 * b]);
+                            acc[x][2 * b + 1] = mfma(hi, pl[x][y], acc[x][2 * b + 1]);
                         }
                     }
-                load_v(next, vnext, z);
-            }
+                }
+            load_v(next, vnext);
         }
         // the next piece's loads are on their way while this one is put together
         const Tile done = t;
@@ -849,7 +846,10 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
         if (!whole_tile<R>(a, t)) return;
         work.left = 0;
     } else if constexpr (SPLIT) {
-        if (!work_of<R>(a, work, batch, blockIdx.x, gridDim.x)) return;
+        if (!work_of<R>(a, work, batch, blockIdx.x, gridDim.x)) {
+            if (threadIdx.x == 0) *left_of(a, blockIdx.x) = Left{};
+            return;
+        }
     }
     const int ps = 1 << a.c.ps_shift;
     const int kt = wave & 3, s0 = W == 8 ? (wave >> 2) * KW : 0, j0 = wave * NJ;
@@ -1083,6 +1083,8 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
         if (n + 1 < units) turn(n + 1, d, c);
     }
     const Shared sh = one ? Shared{0, 0} : shared_of(work, part);
+    if (SPLIT && !one && work.left == 0 && threadIdx.x == 0)  // (a block's last piece is the one that others may share)
+        *left_of(a, blockIdx.x) = sh.split() && sh.b0 == (int)blockIdx.x ? Left{t.q0, t.head, t.r0, t.r1, sh.b1, {}} : Left{};
 #pragma unroll
     for (int x = 0; x < NT; x++) {
         const float l = sum[x][0];
@@ -1104,22 +1106,16 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
 }
 
 // The shared tiles of 64 rows to one, in a launch of its own: block (b, s) has
-// some rows of the tile that block b of `blocks` left unfinished, if it was the
-// first on it, one a lane group.  (By the block that finishes last, as above, one block read all
+// some rows of the tile that block b was the first on and left unfinished, one
+// a lane group.  (By the block that finishes last, as above, one block read all
 // parts of 64 rows: 16 rows a sequence of 9000 keys, 8 sequences, 64 us.)
 template <int HD, bool F16, int R>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a, int blocks) {
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR, PB = 8;  // (eight blocks' parts in flight)
-    Work work;
-    Batch batch;
-    if (!work_of<R>(a, work, batch, blockIdx.x, blocks)) return;
+    const Left left = *left_of(a, blockIdx.x);
+    const Shared sh = {(int)blockIdx.x, left.b1};
     Tile t;
-    Units u;
-    Piece part;
-    do piece_of<R>(a, work, batch, t, u, part);
-    while (work.left > 0);
-    const Shared sh = shared_of(work, part);
-    if (!sh.split() || sh.b0 != (int)blockIdx.x) return;
+    t.q0 = left.q0, t.head = left.head, t.r0 = left.r0, t.r1 = left.r1;
     const int l = threadIdx.x % LPR, r = t.r0 + (int)blockIdx.y * RPB + threadIdx.x / LPR;
     if (r < t.r1) {
         float m = __builtin_inff(), sum = 0.0f;
@@ -1151,14 +1147,14 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid);
     constexpr int NT = HD == 64 || (HD == 128 && F16) ? 2 : 1;  // row tiles a wave of the large tiles
     if (p.rows == 16) {
-        hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, HD == 256 ? 2 : 1, 1>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, 1>), grid, dim3(256), 0, st, a);
     } else if (HD == 128 && p.rows == 32) {
-        hipLaunchKernelGGL((k_kv4_attn<128, F16, 4, 1, 2>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_kv4_attn<128, F16, 4, 2>), grid, dim3(256), 0, st, a);
     } else if (p.rows == 64) {
         hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 4, 1, true>), grid, dim3(256), 0, st, a);
         if (p.whole) return;
         constexpr int RPB = 256 / (HD / 4);
-        hipLaunchKernelGGL((k_kv4_join<HD, F16, 64>), dim3((unsigned)p.grid, 64 / RPB), dim3(256), 0, st, a, (int)p.grid);
+        hipLaunchKernelGGL((k_kv4_join<HD, F16, 64>), dim3((unsigned)p.grid, 64 / RPB), dim3(256), 0, st, a);
     } else if constexpr (HD != 256 || F16) {
         hipLaunchKernelGGL((k_kv4_attn_prompt<HD, F16, 8, NT, false>), grid, dim3(512), 0, st, a);
     }
@@ -1186,7 +1182,14 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
 //   300: 15 against 31 split); else equal stretches of their units for two
 //   blocks a CU (one at head dim 256, whose operands fill the LDS), and the
 //   join's launch: 300 rows over 5000 keys 62 against 90 whole.
-Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, int cus) {
+// A block takes `chunk` units at least.  Of a tile of n units the decode kernel's
+// blocks go through chunk / 4 turns and its last one through n / chunk parts
+// of 4 a turn, each a round trip: least near sqrt(2 n), a multiple of the 4
+// waves (one token over 10000 keys, 32 / 4 heads of 128: 27 us, 42 at 4 units
+// always; over 100000 keys of 64 38 against 48).  The join's launch reads all
+// parts at once: 2 (4 drafts of 30 rows over 700 keys of 256 29 us, 33 at 4).
+Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, int n_kv, int max_q, long max_keys,
+                          int cus) {
     Kv4AttnPlan p = {};
     const int group = n_head / n_kv;
     const int big = hd == 64 || (hd == 128 && f16) ? 256 : hd == 256 && !f16 ? 64 : 128;
@@ -1196,15 +1199,15 @@ Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, in
     if (hd == 128 && p.rows == 64 && rows <= 32) p.rows = 32;
     p.whole = p.rows > 64 || (p.rows == 64 && tiles(64) >= cus);
     p.grid = p.whole ? ((long)n_tok * group / p.rows + n_seq) * n_kv : (p.rows != 32 && hd != 256 ? 2 : 1) * cus;
-    p.chunk = p.rows <= 32 ? 4 : 2;  // (a unit for each of the decode kernel's waves)
+    p.chunk = p.rows <= 32 ? 4 * (int)fmax(1.0, 0.25 * sqrt(2.0 * (double)max_keys / UNIT) + 0.5) : 2;
     p.part_bytes = p.whole ? 0 : (size_t)p.grid * 2 * p.rows * (hd + 4) * sizeof(float);
-    p.work = p.whole ? 0 : KV4_COUNT_BYTES + p.part_bytes;
+    p.work = p.whole ? 0 : KV4_COUNT_BYTES + p.part_bytes + (p.rows == 64 ? p.grid * sizeof(Left) : 0);
     return p;
 }
 
 // Of split tiles of 64 rows, the most of any plan.
 size_t kv4_attn_workspace(int hd, int cus) {
-    return KV4_COUNT_BYTES + (size_t)(hd != 256 ? 2 : 1) * cus * 2 * 64 * (hd + 4) * sizeof(float);
+    return KV4_COUNT_BYTES + (size_t)(hd != 256 ? 2 : 1) * cus * (2 * 64 * (hd + 4) * sizeof(float) + sizeof(Left));
 }
 
 int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, void* work, hipStream_t st) {

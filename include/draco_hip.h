@@ -603,9 +603,8 @@ int draco_kv4_read(const DracoKv4* cache, const int* slot, int n, float* k, floa
  * draco_kv4_append (out must not be q).  One call serves decode (one row a
  * sequence), drafts and prompt chunks, mixed as they come.
  *
- * max_q: the largest row count of a sequence, or more; a smaller value only
- * costs speed.  max_len: the largest length, or more (0 or more; nothing
- * depends on it now).  A length past max_blocks pages, a page outside the pool
+ * max_q, max_len: the largest row count and length of a sequence; other values
+ * only cost speed.  A length past max_blocks pages, a page outside the pool
  * that a row sees, or a score past fp32's range gives NaN.
  *
  * work / work_bytes: draco_kv4_attn_workspace(cache, p) bytes, 16-byte
