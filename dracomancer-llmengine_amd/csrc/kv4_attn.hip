@@ -647,12 +647,18 @@ __device__ __forceinline__ void join_waves(f4v* acc, float nfm, float& l, float*
 }
 
 // Up to 16 NT rows of a sequence and KV head (decode, a few drafts): a block's
-// waves take the units of its piece in turn.  A wave's K words are free once the scores
-// are done and its V words once the output is: the loads of the wave's next
-// unit go there and then.  V scales (a lane's operands need all 16 of
-// its tokens', the same for 16 lanes) come as one 64th a lane and pass through
-// LDS, which takes 8 wide loads and 32 registers less than loading them to
-// every lane.
+// waves take the units of its piece in turn, each straight into registers.  A
+// wave's K words are free once the scores are done and its V words once the
+// output is: the loads of the wave's next unit go there and then.  V scales (a
+// lane's operands need all 16 of its tokens', the same for 16 lanes) come as
+// one 64th a lane and pass through LDS, which takes 8 wide loads and 32
+// registers less than loading them to every lane.
+// HBM bound where the batch is long: 64 sequences of up to 16384 keys, 32 / 4
+// heads of 128, fp32 rows, 395 MB in 95 us (4.15 TB/s; a copy reaches 4.80).
+// Short ones are a chain of latencies: 1000 keys of 32 / 8 heads of 64 9 us.
+// One unit in flight a wave: two made hardly more of the bandwidth and much
+// more code, which every block fetches first (24 sequences of 16 / 2 heads of
+// 256, window 6001: 41 us against 47).
 template <int HD>
 struct Raw {
     KRow<HD, HD / 32> k[4];
@@ -830,6 +836,10 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
 // exponentials of unit n among the products of unit n + 1's scores, and stages
 // later units' operands among unit n's output products.  K operands are staged
 // two units ahead and V operands one; one barrier a turn.
+// Bound by the matrix units and the vector work beside them: 2048 rows of 32 /
+// 4 heads of 128 over 8192 keys, f16, 265-273 us (880-909 TFLOP/s, a library
+// product of 8192^3 1123); five prompts of 777, window 500, 32 / 8 heads of
+// 64, fp32 rows, 42 us (an exponential costs there what a score's products do).
 template <int HD, bool F16, int W, int NT, bool SPLIT>
 __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
     constexpr int KS = HD / 32, MT = HD / 16, R = 16 * NT * W;
@@ -854,261 +864,263 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
     const int ps = 1 << a.c.ps_shift;
     const int kt = wave & 3, s0 = W == 8 ? (wave >> 2) * KW : 0, j0 = wave * NJ;
     const bool stage_v = j0 < 2 * KS;
-  do {
-    Units u;
-    Piece part;
-    if (one) {
-        u = tile_units(a, t, t.r0, t.r1);
-        part.lo = 0;
-        part.hi = u.n;
-    } else if constexpr (SPLIT) {
-        piece_of<R>(a, work, batch, t, u, part);
-    }
-    const int units = part.hi - part.lo;
-    __syncthreads();  // the last piece's operands are read
-    KRow<HD, KW> k;
-    VPart v[NJ];
-    int kp, vp;  // pages of the units to load next
-    bool v_ok = true;
-    // (past the end the last unit again: no branch around loads)
-    auto unit_of = [&](int n) { return u.at(max(min(part.lo + n, part.hi - 1), 0)); };
-    auto load_k = [&](int n) {  // unit n's K codes, and the page of unit n + 1
-        bool ok;
-        const int key = k_key(unit_of(n));
-        const uint8_t* p = page_ptr(a, kp, key, t.head, ok);
-        load_krow<HD, KW>(p, ok, ps, (key & (ps - 1)) + 4 * kt, s0, k);
-        kp = page_of(a, t.table, k_key(unit_of(n + 1)));
-    };
-    auto load_v = [&](int n) {
-        const int key = v_key(unit_of(n));
-        const uint8_t* p = page_ptr(a, vp, key, t.head, v_ok);
-#pragma unroll
-        for (int j = 0; j < NJ; j++) load_vpart<HD>(p, ps, key & (ps - 1), ((j0 + j) >> 1) & (KS - 1), (j0 + j) & 1, v[j]);
-        vp = page_of(a, t.table, v_key(unit_of(n + 1)));
-    };
-    auto stage_k = [&](int n) {
-        h8v* bk = s_k[n & 1];
-#pragma unroll
-        for (int s = 0; s < KW; s++) bk[((s0 + s) * 4 + kt) * 64 + lane] = k_operand(k.w[s], k.scale(s));
-    };
-    auto cut_v = [&](int n) {
-        const int key0 = unit_of(n) * UNIT;
-        if (key0 + UNIT > t.len || !v_ok) {
-#pragma unroll
-            for (int j = 0; j < NJ; j++) cut_vpart(v[j], key0 + 16 * g + 8 * ((j0 + j) & 1), v_ok ? t.len : 0);
+    do {
+        Units u;
+        Piece part;
+        if (one) {
+            u = tile_units(a, t, t.r0, t.r1);
+            part.lo = 0;
+            part.hi = u.n;
+        } else if constexpr (SPLIT) {
+            piece_of<R>(a, work, batch, t, u, part);
         }
-    };
-    auto stage_v_ops = [&](int n) {
-        h8v* bv = s_v[n & 1];
+        const int units = part.hi - part.lo;
+        __syncthreads();  // the last piece's operands are read
+        KRow<HD, KW> k;
+        VPart v[NJ];
+        int kp, vp;  // pages of the units to load next
+        bool v_ok = true;
+        // (past the end the last unit again: no branch around loads)
+        auto unit_of = [&](int n) { return u.at(max(min(part.lo + n, part.hi - 1), 0)); };
+        auto load_k = [&](int n) {  // unit n's K codes, and the page of unit n + 1
+            bool ok;
+            const int key = k_key(unit_of(n));
+            const uint8_t* p = page_ptr(a, kp, key, t.head, ok);
+            load_krow<HD, KW>(p, ok, ps, (key & (ps - 1)) + 4 * kt, s0, k);
+            kp = page_of(a, t.table, k_key(unit_of(n + 1)));
+        };
+        auto load_v = [&](int n) {
+            const int key = v_key(unit_of(n));
+            const uint8_t* p = page_ptr(a, vp, key, t.head, v_ok);
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            h8v lo, hi;
-            v_operands(v[j], lo, hi);
-            if (2 * KS >= W || stage_v) {
-                bv[((j0 + j) * 2 + 0) * 64 + lane] = lo;
-                bv[((j0 + j) * 2 + 1) * 64 + lane] = hi;
+            for (int j = 0; j < NJ; j++) load_vpart<HD>(p, ps, key & (ps - 1), ((j0 + j) >> 1) & (KS - 1), (j0 + j) & 1, v[j]);
+            vp = page_of(a, t.table, v_key(unit_of(n + 1)));
+        };
+        auto stage_k = [&](int n) {
+            h8v* bk = s_k[n & 1];
+#pragma unroll
+            for (int s = 0; s < KW; s++) bk[((s0 + s) * 4 + kt) * 64 + lane] = k_operand(k.w[s], k.scale(s));
+        };
+        auto cut_v = [&](int n) {
+            const int key0 = unit_of(n) * UNIT;
+            if (key0 + UNIT > t.len || !v_ok) {
+#pragma unroll
+                for (int j = 0; j < NJ; j++) cut_vpart(v[j], key0 + 16 * g + 8 * ((j0 + j) & 1), v_ok ? t.len : 0);
             }
+        };
+        auto stage_v_ops = [&](int n) {
+            h8v* bv = s_v[n & 1];
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                h8v lo, hi;
+                v_operands(v[j], lo, hi);
+                if (2 * KS >= W || stage_v) {
+                    bv[((j0 + j) * 2 + 0) * 64 + lane] = lo;
+                    bv[((j0 + j) * 2 + 1) * 64 + lane] = hi;
+                }
+            }
+        };
+        kp = page_of(a, t.table, k_key(unit_of(0)));
+        vp = page_of(a, t.table, v_key(unit_of(0)));
+        // this wave's rows; a wave without any repeats the tile's last and stores nothing
+        const int r0 = min(t.r0 + wave * 16 * NT, t.r1 - 1), r1 = min(t.r0 + (wave + 1) * 16 * NT, t.r1);
+        h8v qh[NT][KS], ql[NT][F16 ? 1 : KS];
+        Row w[NT];
+        f4v acc[NT][MT], c[NT][4], d[NT][4];
+#pragma unroll
+        for (int x = 0; x < NT; x++) {
+            const int r = min(r0 + 16 * x + i, t.r1 - 1);
+            float f;
+            load_q<HD, F16>(a, t, r, qh[x], ql[x], f);
+            row_init(a, t, r, f, w[x]);
+#pragma unroll
+            for (int m = 0; m < MT; m++) acc[x][m] = f4v{0, 0, 0, 0};
         }
-    };
-    kp = page_of(a, t.table, k_key(unit_of(0)));
-    vp = page_of(a, t.table, v_key(unit_of(0)));
-    // this wave's rows; a wave without any repeats the tile's last and stores nothing
-    const int r0 = min(t.r0 + wave * 16 * NT, t.r1 - 1), r1 = min(t.r0 + (wave + 1) * 16 * NT, t.r1);
-    h8v qh[NT][KS], ql[NT][F16 ? 1 : KS];
-    Row w[NT];
-    f4v acc[NT][MT], c[NT][4], d[NT][4];
+        const Whole whole = whole_of(a, t, r0, max(r1, r0 + 1));
+        load_k(0);
+        load_v(0);
+        stage_k(0);
+        cut_v(0);
+        stage_v_ops(0);
+        load_k(1);
+        load_v(1);
+        stage_k(1);
+        load_k(2);
+        lds_barrier();
+        // Operands are read one step ahead of their products, and each step's
+        // products have a share of the vector work between them: left to itself the
+        // compiler reads an operand where it is used and waits out the LDS.
+        h8v cur[4], nxt[4];
+        auto read = [&](const h8v* p, h8v (&o)[4]) {
 #pragma unroll
-    for (int x = 0; x < NT; x++) {
-        const int r = min(r0 + 16 * x + i, t.r1 - 1);
-        float f;
-        load_q<HD, F16>(a, t, r, qh[x], ql[x], f);
-        row_init(a, t, r, f, w[x]);
-#pragma unroll
-        for (int m = 0; m < MT; m++) acc[x][m] = f4v{0, 0, 0, 0};
-    }
-    const Whole whole = whole_of(a, t, r0, max(r1, r0 + 1));
-    load_k(0);
-    load_v(0);
-    stage_k(0);
-    cut_v(0);
-    stage_v_ops(0);
-    load_k(1);
-    load_v(1);
-    stage_k(1);
-    load_k(2);
-    lds_barrier();
-    // Operands are read one step ahead of their products, and each step's
-    // products have a share of the vector work between them: left to itself the
-    // compiler reads an operand where it is used and waits out the LDS.
-    h8v cur[4], nxt[4];
-    auto read = [&](const h8v* p, h8v (&o)[4]) {
-#pragma unroll
-        for (int y = 0; y < 4; y++) o[y] = p[y * 64 + lane];
-    };
-    auto products = [&](int e, f4v (&s)[NT][4]) {
-#pragma unroll
-        for (int y = 0; y < 4; y++)
-#pragma unroll
-            for (int x = 0; x < NT; x++) s[x][y] = mfma(cur[y], qh[x][e], s[x][y]);
-        if constexpr (!F16) {
+            for (int y = 0; y < 4; y++) o[y] = p[y * 64 + lane];
+        };
+        auto products = [&](int e, f4v (&s)[NT][4]) {
 #pragma unroll
             for (int y = 0; y < 4; y++)
 #pragma unroll
-                for (int x = 0; x < NT; x++) s[x][y] = mfma(cur[y], ql[x][e], s[x][y]);
-        }
-    };
-    auto clear = [&](f4v (&s)[NT][4]) {
+                for (int x = 0; x < NT; x++) s[x][y] = mfma(cur[y], qh[x][e], s[x][y]);
+            if constexpr (!F16) {
 #pragma unroll
-        for (int x = 0; x < NT; x++)
+                for (int y = 0; y < 4; y++)
 #pragma unroll
-            for (int y = 0; y < 4; y++) s[x][y] = f4v{0, 0, 0, 0};
-    };
-    constexpr int NM = 4 * NT * (F16 ? 1 : 2);  // products of a step
-    auto interleave = [&](auto vec) {           // .. with vec.value vector instructions behind each
-#pragma unroll
-        for (int m = 0; m < NM; m++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, decltype(vec)::value, 0);
-        }
-    };
-    clear(c);
-#pragma unroll
-    for (int e = 0; e < KS; e++) {
-        read(s_k[0] + e * 256, cur);
-        products(e, c);
-    }
-    lds_barrier();  // unit 0's K buffer goes to unit 2
-    // Sums of the rounded p, by products with ones (a lane's column is its row):
-    // less work than adding, and the weights that are applied sum to one.
-    f4v sum[NT];
-    h8v ones;
-#pragma unroll
-    for (int e = 0; e < 8; e++) ones[e] = (_Float16)1.0f;
-#pragma unroll
-    for (int x = 0; x < NT; x++) sum[x] = f4v{w[x].l, w[x].l, w[x].l, w[x].l};
-    auto turn = [&](int n, f4v (&c)[NT][4], f4v (&d)[NT][4]) {
-        const int key0 = unit_of(n) * UNIT;
-        const bool all = whole.has(key0);
-        const h8v *bk = s_k[(n + 1) & 1], *bv = s_v[n & 1];
-        read(bk, cur);
-        float top[NT];
-        if (all) {
-#pragma unroll
-            for (int x = 0; x < NT; x++) top[x] = row_max<false>(w[x], key0 + 16 * g, a.sink, c[x]);
-        } else {
-#pragma unroll
-            for (int x = 0; x < NT; x++) top[x] = row_max<true>(w[x], key0 + 16 * g, a.sink, c[x]);
-        }
-        bool grow = false;
-#pragma unroll
-        for (int x = 0; x < NT; x++) grow |= grows(w[x], top[x]);
-        if (__any(grow)) {
-#pragma unroll
-            for (int x = 0; x < NT; x++) {
-                const float keep = follow<MT>(w[x], top[x], acc[x]);
-                sum[x] *= keep;
+                    for (int x = 0; x < NT; x++) s[x][y] = mfma(cur[y], ql[x][e], s[x][y]);
             }
-        }
-        cut_v(n + 1);
-        // scores of unit n + 1, probabilities of unit n
-        h8v ph[NT][2], pl[NT][2];
-        clear(d);
+        };
+        auto clear = [&](f4v (&s)[NT][4]) {
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) s[x][y] = f4v{0, 0, 0, 0};
+        };
+        constexpr int NM = 4 * NT * (F16 ? 1 : 2);  // products of a step
+        auto interleave = [&](auto vec) {           // .. with vec.value vector instructions behind each
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, decltype(vec)::value, 0);
+            }
+        };
+        clear(c);
 #pragma unroll
         for (int e = 0; e < KS; e++) {
-            read(e + 1 < KS ? bk + (e + 1) * 256 : bv, nxt);
-            __builtin_amdgcn_sched_barrier(0);
-            products(e, d);
-#pragma unroll
-            for (int y = e * 4 / KS; y < (e + 1) * 4 / KS; y++)
-#pragma unroll
-                for (int x = 0; x < NT; x++)
-#pragma unroll
-                    for (int z = 0; z < 4; z++) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y][z], w[x].f, w[x].nfm));
-                        const int at = 4 * (y & 1) + z;
-                        ph[x][y >> 1][at] = (_Float16)p;
-                        if constexpr (!F16) pl[x][y >> 1][at] = (_Float16)__builtin_fmaf((float)ph[x][y >> 1][at], -1.0f, p);
-                    }
-            interleave(std::integral_constant<int, 16 * NT * (F16 ? 3 : 5) / KS / NM>());
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < 4; y++) cur[y] = nxt[y];
+            read(s_k[0] + e * 256, cur);
+            products(e, c);
         }
-        // output of unit n; operands of units n + 2 and n + 1, codes of the units after them
+        lds_barrier();  // unit 0's K buffer goes to unit 2
+        // Sums of the rounded p, by products with ones (a lane's column is its row):
+        // less work than adding, and the weights that are applied sum to one.
+        f4v sum[NT];
+        h8v ones;
 #pragma unroll
-        for (int b = 0; b < KS; b++) {
-            if (b + 1 < KS) read(bv + (b + 1) * 256, nxt);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 8; e++) ones[e] = (_Float16)1.0f;
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
+        for (int x = 0; x < NT; x++) sum[x] = f4v{w[x].l, w[x].l, w[x].l, w[x].l};
+        auto turn = [&](int n, f4v (&c)[NT][4], f4v (&d)[NT][4]) {
+            const int key0 = unit_of(n) * UNIT;
+            const bool all = whole.has(key0);
+            const h8v *bk = s_k[(n + 1) & 1], *bv = s_v[n & 1];
+            read(bk, cur);
+            float top[NT];
+            if (all) {
+#pragma unroll
+                for (int x = 0; x < NT; x++) top[x] = row_max<false>(w[x], key0 + 16 * g, a.sink, c[x]);
+            } else {
+#pragma unroll
+                for (int x = 0; x < NT; x++) top[x] = row_max<true>(w[x], key0 + 16 * g, a.sink, c[x]);
+            }
+            bool grow = false;
+#pragma unroll
+            for (int x = 0; x < NT; x++) grow |= grows(w[x], top[x]);
+            if (__any(grow)) {
 #pragma unroll
                 for (int x = 0; x < NT; x++) {
-                    acc[x][2 * b] = mfma(cur[2 * y], ph[x][y], acc[x][2 * b]);
-                    acc[x][2 * b + 1] = mfma(cur[2 * y + 1], ph[x][y], acc[x][2 * b + 1]);
+                    const float keep = follow<MT>(w[x], top[x], acc[x]);
+                    sum[x] *= keep;
                 }
-                if constexpr (!F16) {
+            }
+            cut_v(n + 1);
+            // scores of unit n + 1, probabilities of unit n
+            h8v ph[NT][2], pl[NT][2];
+            clear(d);
+#pragma unroll
+            for (int e = 0; e < KS; e++) {
+                read(e + 1 < KS ? bk + (e + 1) * 256 : bv, nxt);
+                __builtin_amdgcn_sched_barrier(0);
+                products(e, d);
+#pragma unroll
+                for (int y = e * 4 / KS; y < (e + 1) * 4 / KS; y++)
+#pragma unroll
+                    for (int x = 0; x < NT; x++)
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y][z], w[x].f, w[x].nfm));
+                            const int at = 4 * (y & 1) + z;
+                            ph[x][y >> 1][at] = (_Float16)p;
+                            if constexpr (!F16) pl[x][y >> 1][at] = (_Float16)__builtin_fmaf((float)ph[x][y >> 1][at], -1.0f, p);
+                        }
+                interleave(std::integral_constant<int, 16 * NT * (F16 ? 3 : 5) / KS / NM>());
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int y = 0; y < 4; y++) cur[y] = nxt[y];
+            }
+            // output of unit n; operands of units n + 2 and n + 1, codes of the units after them
+#pragma unroll
+            for (int b = 0; b < KS; b++) {
+                if (b + 1 < KS) read(bv + (b + 1) * 256, nxt);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
 #pragma unroll
                     for (int x = 0; x < NT; x++) {
-                        acc[x][2 * b] = mfma(cur[2 * y], pl[x][y], acc[x][2 * b]);
-                        acc[x][2 * b + 1] = mfma(cur[2 * y + 1], pl[x][y], acc[x][2 * b + 1]);
+                        acc[x][2 * b] = mfma(cur[2 * y], ph[x][y], acc[x][2 * b]);
+                        acc[x][2 * b + 1] = mfma(cur[2 * y + 1], ph[x][y], acc[x][2 * b + 1]);
+                    }
+                    if constexpr (!F16) {
+#pragma unroll
+                        for (int x = 0; x < NT; x++) {
+                            acc[x][2 * b] = mfma(cur[2 * y], pl[x][y], acc[x][2 * b]);
+                            acc[x][2 * b + 1] = mfma(cur[2 * y + 1], pl[x][y], acc[x][2 * b + 1]);
+                        }
                     }
                 }
-            }
-            if (b == 0) {
-                stage_k(n + 2);
-                load_k(n + 3);
-            }
-            if (b == KS / 2) {
-                stage_v_ops(n + 1);
-                load_v(n + 2);
-            }
-            if (b == KS - 1) {
+                if (b == 0) {
+                    stage_k(n + 2);
+                    load_k(n + 3);
+                }
+                if (b == KS / 2) {
+                    stage_v_ops(n + 1);
+                    load_v(n + 2);
+                }
+                if (b == KS - 1) {
 #pragma unroll
-                for (int x = 0; x < NT; x++)
+                    for (int x = 0; x < NT; x++)
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        sum[x] = mfma(ones, ph[x][y], sum[x]);
-                        if constexpr (!F16) sum[x] = mfma(ones, pl[x][y], sum[x]);
-                    }
+                        for (int y = 0; y < 2; y++) {
+                            sum[x] = mfma(ones, ph[x][y], sum[x]);
+                            if constexpr (!F16) sum[x] = mfma(ones, pl[x][y], sum[x]);
+                        }
+                }
+                interleave(std::integral_constant<int, 4>());
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int y = 0; y < 4; y++) cur[y] = nxt[y];
             }
-            interleave(std::integral_constant<int, 4>());
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < 4; y++) cur[y] = nxt[y];
+            lds_barrier();
+        };
+        for (int n = 0; n < units; n += 2) {  // (two turns: the scores change places without copies)
+            turn(n, c, d);
+            if (n + 1 < units) turn(n + 1, d, c);
         }
-        lds_barrier();
-    };
-    for (int n = 0; n < units; n += 2) {  // (two turns: the scores change places without copies)
-        turn(n, c, d);
-        if (n + 1 < units) turn(n + 1, d, c);
-    }
-    const Shared sh = one ? Shared{0, 0} : shared_of(work, part);
-    if (SPLIT && !one && work.left == 0 && threadIdx.x == 0)  // (a block's last piece is the one that others may share)
-        *left_of(a, blockIdx.x) = sh.split() && sh.b0 == (int)blockIdx.x ? Left{t.q0, t.head, t.r0, t.r1, sh.b1, {}} : Left{};
+        const Shared sh = one ? Shared{0, 0} : shared_of(work, part);
+        if (SPLIT && !one && work.left == 0 && threadIdx.x == 0)  // (a block's last piece is the one that others may share)
+            *left_of(a, blockIdx.x) = sh.split() && sh.b0 == (int)blockIdx.x ? Left{t.q0, t.head, t.r0, t.r1, sh.b1, {}} : Left{};
 #pragma unroll
-    for (int x = 0; x < NT; x++) {
-        const float l = sum[x][0];
-        const int r = r0 + 16 * x + i;
-        if (r >= r1) continue;
-        if (!sh.split()) {
-            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-            const long at = out_at(a, t, r, HD);
+        for (int x = 0; x < NT; x++) {
+            const float l = sum[x][0];
+            const int r = r0 + 16 * x + i;
+            if (r >= r1) continue;
+            if (!sh.split()) {
+                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+                const long at = out_at(a, t, r, HD);
 #pragma unroll
-            for (int m = 0; m < MT; m++) store4<F16>(a, at + 16 * m + 4 * g, acc[x][m] * inv);
-        } else {
-            float* row = a.part + part_at<HD, R>(sh.slot(blockIdx.x), r - t.r0);
+                for (int m = 0; m < MT; m++) store4<F16>(a, at + 16 * m + 4 * g, acc[x][m] * inv);
+            } else {
+                float* row = a.part + part_at<HD, R>(sh.slot(blockIdx.x), r - t.r0);
 #pragma unroll
-            for (int m = 0; m < MT; m++) *(f4v*)(row + 16 * m + 4 * g) = acc[x][m];
-            if (g == 0) *(f4v*)(row + HD) = f4v{l, w[x].nfm, 0, 0};
+                for (int m = 0; m < MT; m++) *(f4v*)(row + 16 * m + 4 * g) = acc[x][m];
+                if (g == 0) *(f4v*)(row + HD) = f4v{l, w[x].nfm, 0, 0};
+            }
         }
-    }
-  } while (SPLIT && work.left > 0);
+    } while (SPLIT && work.left > 0);
 }
 
 // The shared tiles of 64 rows to one, in a launch of its own: block (b, s) has
 // some rows of the tile that block b was the first on and left unfinished, one
 // a lane group.  (By the block that finishes last, as above, one block read all
-// parts of 64 rows: 16 rows a sequence of 9000 keys, 8 sequences, 64 us.)
+// parts of 64 rows: 16 rows a sequence of 9000 keys, 8 sequences, 64 us, now 48.
+// With the record of `Left` a block knows its tile after one read: 24 sequences
+// of 5 rows, window 6001, 16 / 2 heads of 256 8 us, 17 where it searched.)
 template <int HD, bool F16, int R>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR, PB = 8;  // (eight blocks' parts in flight)
