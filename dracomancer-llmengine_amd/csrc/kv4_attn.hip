@@ -1194,6 +1194,11 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
 //   300: 15 against 31 split); else equal stretches of their units for two
 //   blocks a CU (one at head dim 256, whose operands fill the LDS), and the
 //   join's launch: 300 rows over 5000 keys 62 against 90 whole.
+// - the decode kernel at head dims 64 and 128: two blocks a CU where the batch
+//   has tiles or units for them (64 sequences of 1000 keys, 8 KV heads of 128
+//   32 against 45 with one; 64 of 16384 95 against 112), else one, whose longer
+//   stretches leave fewer parts to join (20 of 3000, 8 KV heads of 128 25
+//   against 29; 24 windows of 6001, 4 KV heads 31 against 35).
 // A block takes `chunk` units at least.  Of a tile of n units the decode kernel's
 // blocks go through chunk / 4 turns and its last one through n / chunk parts
 // of 4 a turn, each a round trip: least near sqrt(2 n), a multiple of the 4
@@ -1210,7 +1215,9 @@ Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, in
     p.rows = rows <= 16 ? 16 : rows > 64 && 2 * tiles(big) >= (hd == 64 ? 4 : hd == 128 ? 2 : 1) * cus ? big : 64;
     if (hd == 128 && p.rows == 64 && rows <= 32) p.rows = 32;
     p.whole = p.rows > 64 || (p.rows == 64 && tiles(64) >= cus);
-    p.grid = p.whole ? ((long)n_tok * group / p.rows + n_seq) * n_kv : (p.rows != 32 && hd != 256 ? 2 : 1) * cus;
+    const long decode = (long)n_seq * n_kv;  // tiles of the decode kernel
+    const bool two = hd != 256 && (p.rows == 64 || (p.rows == 16 && (3 * decode >= 2 * cus || (double)decode * max_keys >= 64.0 * UNIT * cus)));
+    p.grid = p.whole ? ((long)n_tok * group / p.rows + n_seq) * n_kv : (two ? 2 : 1) * cus;
     p.chunk = p.rows <= 32 ? 4 * (int)fmax(1.0, 0.25 * sqrt(2.0 * (double)max_keys / UNIT) + 0.5) : 2;
     p.part_bytes = p.whole ? 0 : (size_t)p.grid * 2 * p.rows * (hd + 4) * sizeof(float);
     p.work = p.whole ? 0 : KV4_COUNT_BYTES + p.part_bytes + (p.rows == 64 ? p.grid * sizeof(Left) : 0);
