@@ -452,6 +452,18 @@ def test_attn_many_sequences(dev, hd, nh, nkv, code, most):
     check_sampled(Cache(dev, lens, nkv, hd, 16), lens, qlens, nh, rng, code, 40 if most == 4 else 0, 3, 60)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("code", [F32, F16])
+@pytest.mark.parametrize("most", [1, 7, 15, 40])
+@pytest.mark.parametrize("window,sink", [(0, 0), (33, 0), (100, 5), (1, 1), (1000, 200)])
+def test_attn_masks_of_every_kernel(dev, hd, code, most, window, sink):
+    """Partly masked units (ends, window starts, sinks) in each kernel: 4, 28, 60 and 160 rows a KV head."""
+    rng = np.random.default_rng(hd + most + window)
+    lens, qlens = [63, 321, most, 200 + most], [1, most, most, max(1, most - 1)]
+    c = Cache(dev, lens, 1, hd, 16)
+    check_attn(c, fill(c, lens, rng, code), lens, qlens, 4, rng, code, window=window, sink=sink)
+
+
 @pytest.mark.parametrize("hd,code", [(64, F32), (128, F16)])
 @pytest.mark.parametrize("n_seq", [300, 4500])
 def test_attn_whole_tiles_of_many_sequences(dev, hd, code, n_seq):
