@@ -166,7 +166,7 @@ __device__ __forceinline__ bool work_of(const Kv4AttnArgs& a, Work& w, Batch& b,
     w.left = (int)min((long)w.chunk, total - w.at);
     if (w.left <= 0) return false;
     long before = 0;
-    for (int s = 0;; s += 64) {
+    for (int s = 0; s < a.n_seq; s += 64) {
         if (a.n_seq > 64) {
             batch_of(a, s, b);
             mine = wave_scan(batch_units<R>(a, b));
@@ -180,6 +180,7 @@ __device__ __forceinline__ bool work_of(const Kv4AttnArgs& a, Work& w, Batch& b,
         }
         before += lane_of(mine, 63);
     }
+    return false;  // (the lengths were written during the call)
 }
 
 // One tile a block, whole (prompts: enough of them, and partial rows of many
@@ -220,6 +221,16 @@ struct Piece {
 template <int R>
 __device__ __forceinline__ void piece_of(const Kv4AttnArgs& a, Work& w, Batch& b, Tile& t, Units& u, Piece& p) {
     for (;; w.seq++) {
+        if (w.seq >= a.n_seq) {  // lengths that are written during the call: a NaN row, and an end
+            t.q0 = min(t.q0, a.n_tok - 1);
+            t.bad = true;
+            t.head = t.r0 = 0;
+            t.r1 = 1;
+            u = {0, 0, 0};
+            p = {0, 0, w.at, 1};
+            w.left = 0;
+            return;
+        }
         seq_of(a, b, w.seq, t);
         p.n = uni(tile_bound<R>(a, t));
         const long tile = (long)p.n * a.c.n_kv, all = (t.rows + R - 1) / R * tile;
