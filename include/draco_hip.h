@@ -475,9 +475,9 @@ int draco_bench_gemv_q8k(int code, const uint8_t* W, int n_out, int n_in, int nv
  * are enqueued on `stream` (a hipStream_t; NULL = the library's own stream, so
  * the legacy default stream cannot be named) and not waited for.  Nothing is
  * allocated and nothing is cleared by memset nodes: calls can be captured, and
- * a replay reads the arrays' values of that time.  An array that a call reads is
- * not written while it runs.  The structs are read before the call returns.  0 ok, -1 unsupported or bad argument (nothing enqueued),
- * -2 device error.
+ * a replay reads the arrays' values of that time.  Nothing else writes an array
+ * while a call reads it.  The structs are read before the call returns.  0 ok,
+ * -1 unsupported or bad argument (nothing enqueued), -2 device error.
  *
  * A value is code * scale: the code E2M1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a
  * sign), one f16 scale per 32 values of a row: the largest magnitude / 6 to 9
