@@ -12,11 +12,9 @@
 // takes them (16 consecutive keys a lane group; the contraction's order is
 // free as long as both operands share it).
 //
-// K and V values are exact in f16 (kv4.h).  fp32 rows: q (scaled by a power of
-// two to [1, 2) of its largest) and p are split into two f16 terms, 22 bits of
-// each, and every product runs twice into one fp32 sum.  f16 rows: q is exact
-// and p is rounded once, to nearest (2^-12 of itself, as the output's own
-// rounding).
+// K and V values are exact in f16 (kv4.h).  p is split into two f16 terms, 22
+// bits, and so is q of fp32 rows (scaled by a power of two to [1, 2) of its
+// largest): their products run twice into one fp32 sum.  q of f16 rows is exact.
 #include <float.h>
 #include <hip/hip_runtime.h>
 
@@ -55,16 +53,35 @@ __device__ __forceinline__ h8v k_operand(uint32_t w, h2v s) {
 
 __device__ __forceinline__ h2v as_h2(uint32_t u) { return __builtin_bit_cast(h2v, u); }
 __device__ __forceinline__ uint32_t as_u(h2v h) { return __builtin_bit_cast(uint32_t, h); }
+__device__ __forceinline__ h8v as_h8(u4v u) { return __builtin_bit_cast(h8v, u); }
 
-// Eight fp32 values as one (F16) or two f16 operands.
-template <bool F16>
+// a and b to f16, and to f16 what that leaves of them: one conversion for both
+// (v_cvt_pk_f16_f32) and one instruction each (v_fma_mixlo_f16, v_fma_mixhi_f16).
+// (Both need values that the compiler knows nothing of: it would turn a product
+// with -1 into a conversion, a subtraction and another conversion, and convert a
+// and b once more.)
+struct Two {
+    uint32_t hi, lo;
+};
+__device__ __forceinline__ Two split2(float a, float b) {
+    typedef float f2v __attribute__((ext_vector_type(2)));
+    uint32_t u = as_u(__builtin_convertvector((f2v{a, b}), h2v));
+    float minus = -1.0f;
+    asm("" : "+v"(u));
+    asm("" : "+s"(minus));
+    const h2v h = as_h2(u);
+    return {u, as_u(h2v{(_Float16)__builtin_fmaf((float)h.x, minus, a), (_Float16)__builtin_fmaf((float)h.y, minus, b)})};
+}
+// Eight fp32 values as two f16 operands.
 __device__ __forceinline__ void split8(const float x[8], h8v& hi, h8v& lo) {
+    u4v h, l;
 #pragma unroll
-    for (int i = 0; i < 8; i++) hi[i] = (_Float16)x[i];
-    if constexpr (!F16) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) lo[i] = (_Float16)__builtin_fmaf((float)hi[i], -1.0f, x[i]);
+    for (int i = 0; i < 4; i++) {
+        const Two t = split2(x[2 * i], x[2 * i + 1]);
+        h[i] = t.hi, l[i] = t.lo;
     }
+    hi = __builtin_bit_cast(h8v, h);
+    lo = __builtin_bit_cast(h8v, l);
 }
 
 // Rows [r0, r1) of one sequence and KV head.
@@ -391,7 +408,7 @@ __device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const Tile& t, int 
         for (int s = 0; s < KS; s++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[s][j] *= up;
-            split8<false>(x[s], hi[s], lo[s]);
+            split8(x[s], hi[s], lo[s]);
         }
         f = a.scale_log2 * __uint_as_float((unsigned)(127 + e) << 23);
     }
@@ -460,7 +477,6 @@ __device__ __forceinline__ float follow(Row& w, float top, f4v* acc) {  // what 
     return keep;
 }
 // Scores to probabilities as the second product's operands.
-template <bool F16>
 __device__ __forceinline__ void probabilities(Row& w, const f4v c[4], h8v ph[2], h8v pl[2]) {
     float p[2][8], sum = 0.0f;
 #pragma unroll
@@ -472,16 +488,16 @@ __device__ __forceinline__ void probabilities(Row& w, const f4v c[4], h8v ph[2],
             sum += e;
         }
     w.l += sum;
-    split8<F16>(p[0], ph[0], pl[0]);
-    split8<F16>(p[1], ph[1], pl[1]);
+    split8(p[0], ph[0], pl[0]);
+    split8(p[1], ph[1], pl[1]);
 }
 // Both, for scores of keys 16 g + 4 t + r of the unit at key0.
-template <bool F16, int MT>
+template <int MT>
 __device__ __forceinline__ void softmax(Row& w, bool whole, int key0, int sink, f4v c[4], f4v* acc, h8v ph[2], h8v pl[2]) {
     const int key = key0 + 16 * ((threadIdx.x & 63) >> 4);
     const float top = whole ? row_max<false>(w, key, sink, c) : row_max<true>(w, key, sink, c);
     if (__any(grows(w, top))) w.l *= follow<MT>(w, top, acc);
-    probabilities<F16>(w, c, ph, pl);
+    probabilities(w, c, ph, pl);
 }
 
 template <bool F16>
@@ -774,7 +790,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
             pages(next + W, kp, vp);
             h8v ph[NT][2], pl[NT][2];
 #pragma unroll
-            for (int x = 0; x < NT; x++) softmax<F16, MT>(w[x], whole.has(key0), key0, a.sink, c[x], acc[x], ph[x], pl[x]);
+            for (int x = 0; x < NT; x++) softmax<MT>(w[x], whole.has(key0), key0, a.sink, c[x], acc[x], ph[x], pl[x]);
             // scales of this lane: tokens 16 g + HD / 32 * (i % (512 / HD)) .. of block i / (512 / HD)
             uint32_t vs[HD / 64];
 #pragma unroll
@@ -802,10 +818,8 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
                     for (int x = 0; x < NT; x++) {
                         acc[x][2 * b] = mfma(lo, ph[x][y], acc[x][2 * b]);
                         acc[x][2 * b + 1] = mfma(hi, ph[x][y], acc[x][2 * b + 1]);
-                        if constexpr (!F16) {
-                            acc[x][2 * b] = mfma(lo, pl[x][y], acc[x][2 * b]);
-                            acc[x][2 * b + 1] = mfma(hi, pl[x][y], acc[x][2 * b + 1]);
-                        }
+                        acc[x][2 * b] = mfma(lo, pl[x][y], acc[x][2 * b]);
+                        acc[x][2 * b + 1] = mfma(hi, pl[x][y], acc[x][2 * b + 1]);
                     }
                 }
             load_v(next, vnext);
@@ -849,10 +863,12 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
 // exponentials of unit n among the products of unit n + 1's scores, and stages
 // later units' operands among unit n's output products.  K operands are staged
 // two units ahead and V operands one; one barrier a turn.
-// Bound by the matrix units and the vector work beside them: 2048 rows of 32 /
-// 4 heads of 128 over 8192 keys, f16, 265-273 us (880-909 TFLOP/s, a library
-// product of 8192^3 1123); five prompts of 777, window 500, 32 / 8 heads of
-// 64, fp32 rows, 42 us (an exponential costs there what a score's products do).
+// 2048 rows of 32 / 4 heads of 128 over 8192 keys: f16 378 us, 361 GFLOP of
+// products issued (p's second term makes them three for two), 954 TFLOP/s, where
+// a library product of 8192^3 reaches 1123; fp32 433 us, 481 GFLOP, 1111.  Two
+// row tiles a wave do not fit the registers there (f16 441 us, 31 spilled).
+// With p as one f16 an f16 call took 273 us, and its rows were off by up to
+// 2^-11 of the values before their own rounding.
 template <int HD, bool F16, int W, int NT, bool SPLIT>
 __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
     constexpr int KS = HD / 32, MT = HD / 16, R = 16 * NT * W;
@@ -986,10 +1002,10 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
 #pragma unroll
                 for (int y = 0; y < 4; y++) s[x][y] = f4v{0, 0, 0, 0};
         };
-        constexpr int NM = 4 * NT * (F16 ? 1 : 2);  // products of a step
-        auto interleave = [&](auto vec) {           // .. with vec.value vector instructions behind each
+        constexpr int QM = 4 * NT * (F16 ? 1 : 2), PM = 8 * NT;  // products of a step: scores, output
+        auto interleave = [&](auto n, auto vec) {                // n.value products, vec.value vector instructions behind each
 #pragma unroll
-            for (int m = 0; m < NM; m++) {
+            for (int m = 0; m < decltype(n)::value; m++) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x002, decltype(vec)::value, 0);
             }
@@ -1034,7 +1050,7 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
             }
             cut_v(n + 1);
             // scores of unit n + 1, probabilities of unit n
-            h8v ph[NT][2], pl[NT][2];
+            u4v ph[NT][2], pl[NT][2];
             clear(d);
 #pragma unroll
             for (int e = 0; e < KS; e++) {
@@ -1046,13 +1062,15 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
 #pragma unroll
                     for (int x = 0; x < NT; x++)
 #pragma unroll
-                        for (int z = 0; z < 4; z++) {
-                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y][z], w[x].f, w[x].nfm));
-                            const int at = 4 * (y & 1) + z;
-                            ph[x][y >> 1][at] = (_Float16)p;
-                            if constexpr (!F16) pl[x][y >> 1][at] = (_Float16)__builtin_fmaf((float)ph[x][y >> 1][at], -1.0f, p);
+                        for (int z = 0; z < 2; z++) {
+                            float p[2];
+#pragma unroll
+                            for (int k = 0; k < 2; k++) p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y][2 * z + k], w[x].f, w[x].nfm));
+                            const Two t = split2(p[0], p[1]);
+                            ph[x][y >> 1][2 * (y & 1) + z] = t.hi;
+                            pl[x][y >> 1][2 * (y & 1) + z] = t.lo;
                         }
-                interleave(std::integral_constant<int, 16 * NT * (F16 ? 3 : 5) / KS / NM>());
+                interleave(std::integral_constant<int, QM>(), std::integral_constant<int, 16 * NT * 5 / KS / QM>());
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int y = 0; y < 4; y++) cur[y] = nxt[y];
@@ -1066,15 +1084,13 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
                 for (int y = 0; y < 2; y++) {
 #pragma unroll
                     for (int x = 0; x < NT; x++) {
-                        acc[x][2 * b] = mfma(cur[2 * y], ph[x][y], acc[x][2 * b]);
-                        acc[x][2 * b + 1] = mfma(cur[2 * y + 1], ph[x][y], acc[x][2 * b + 1]);
+                        acc[x][2 * b] = mfma(cur[2 * y], as_h8(ph[x][y]), acc[x][2 * b]);
+                        acc[x][2 * b + 1] = mfma(cur[2 * y + 1], as_h8(ph[x][y]), acc[x][2 * b + 1]);
                     }
-                    if constexpr (!F16) {
 #pragma unroll
-                        for (int x = 0; x < NT; x++) {
-                            acc[x][2 * b] = mfma(cur[2 * y], pl[x][y], acc[x][2 * b]);
-                            acc[x][2 * b + 1] = mfma(cur[2 * y + 1], pl[x][y], acc[x][2 * b + 1]);
-                        }
+                    for (int x = 0; x < NT; x++) {
+                        acc[x][2 * b] = mfma(cur[2 * y], as_h8(pl[x][y]), acc[x][2 * b]);
+                        acc[x][2 * b + 1] = mfma(cur[2 * y + 1], as_h8(pl[x][y]), acc[x][2 * b + 1]);
                     }
                 }
                 if (b == 0) {
@@ -1090,11 +1106,11 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
                     for (int x = 0; x < NT; x++)
 #pragma unroll
                         for (int y = 0; y < 2; y++) {
-                            sum[x] = mfma(ones, ph[x][y], sum[x]);
-                            if constexpr (!F16) sum[x] = mfma(ones, pl[x][y], sum[x]);
+                            sum[x] = mfma(ones, as_h8(ph[x][y]), sum[x]);
+                            sum[x] = mfma(ones, as_h8(pl[x][y]), sum[x]);
                         }
                 }
-                interleave(std::integral_constant<int, 4>());
+                interleave(std::integral_constant<int, PM>(), std::integral_constant<int, 4>());
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int y = 0; y < 4; y++) cur[y] = nxt[y];
@@ -1170,7 +1186,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
 template <int HD, bool F16>
 void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid);
-    constexpr int NT = HD == 64 || (HD == 128 && F16) ? 2 : 1;  // row tiles a wave of the large tiles
+    constexpr int NT = HD == 64 ? 2 : 1;  // row tiles a wave of the large tiles
     if (p.rows == 16) {
         hipLaunchKernelGGL((k_kv4_attn<HD, F16, 4, 1>), grid, dim3(256), 0, st, a);
     } else if (HD == 128 && p.rows == 32) {
@@ -1193,16 +1209,16 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
 //   nothing but the rows; more rows would read the pages once per 16 of them.
 // - up to 32 at head dim 128 the same with two row tiles (356 registers, so one
 //   block a CU): 24 sequences of 5 drafts over 20011 keys, window 6001, 32 / 8
-//   heads, in fp32 75 against 116 in tiles of 64, 8 of 16 in f16 51 against 54.
+//   heads, 76 against 116 in tiles of 64 in fp32 and 75 against 102 in f16.
 //   At 64 (12 drafts of 32 / 8 heads over 8000 keys 73 against 55) and at 256,
 //   where they spill (5 drafts 98 against 71), the tiles of 64 are faster.
-// - tiles of 64 rows, and of 256 (128 at head dim 128 in fp32 and at 256 in
-//   f16; at 256 in fp32 the registers leave no larger one) where there is one
-//   for every CU: 2048 rows of 32 / 4 heads of 128 over 8192 keys 272 against
-//   351.  At head dim 64, where staging is a smaller part, from two a CU on: five
-//   prompts of 777 46 against 48, one of 8000 (1000 tiles) 595 against 719.  At
-//   256, whose small tiles leave one wave a SIMD, from one for two CUs: 1500 rows
-//   over 3000 keys 116 against 143.
+// - tiles of 64 rows, and of 128 (256 at head dim 64; at 256 in fp32 the
+//   registers leave no larger one) where there is one for every CU: 2048 rows of
+//   32 / 4 heads of 128 over 8192 keys 409 against 435 in f16, 461 against 487 in
+//   fp32.  At head dim 64, where staging is a smaller part, from two a CU on: five
+//   prompts of 777 are as fast either way, one of 8000 (1000 tiles) 584 against
+//   682.  At 256, whose small tiles leave one wave a SIMD, from one for two CUs:
+//   1500 rows over 3000 keys 134 against 158.
 // - tiles whole, one a block, where there is one for every CU (four prompts of
 //   300: 15 against 31 split); else equal stretches of their units for two
 //   blocks a CU (one at head dim 256, whose operands fill the LDS), and the
@@ -1222,7 +1238,7 @@ Kv4AttnPlan kv4_attn_plan(int hd, bool f16, int n_seq, int n_tok, int n_head, in
                           int cus) {
     Kv4AttnPlan p = {};
     const int group = n_head / n_kv;
-    const int big = hd == 64 || (hd == 128 && f16) ? 256 : hd == 256 && !f16 ? 64 : 128;
+    const int big = hd == 64 ? 256 : hd == 256 && !f16 ? 64 : 128;
     const long rows = (long)max_q * group;
     auto tiles = [&](int r) { return (long)n_tok * group / r * n_kv; };
     p.rows = rows <= 16 ? 16 : rows > 64 && 2 * tiles(big) >= (hd == 64 ? 4 : hd == 128 ? 2 : 1) * cus ? big : 64;

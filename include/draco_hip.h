@@ -603,6 +603,10 @@ int draco_kv4_read(const DracoKv4* cache, const int* slot, int n, float* k, floa
  * draco_kv4_append (out must not be q).  One call serves decode (one row a
  * sequence), drafts and prompt chunks, mixed as they come.
  *
+ * Whatever the rows' type and whichever kernel a batch takes: the pages' values
+ * are used as they are, q of fp32 rows and the probabilities in 22 bits, sums
+ * in fp32, and the result is rounded once, to the rows' type.
+ *
  * max_q, max_len: the largest row count and length of a sequence; other values
  * only cost speed.  A length past max_blocks pages, a page outside the pool
  * that a row sees, or a score past fp32's range gives NaN.
