@@ -418,7 +418,7 @@ __device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const Tile& t, int 
 struct Row {
     int pos, lo;    // keys j <= pos, and j >= lo or j < sink
     float f;        // raw score -> exponent of 2
-    float m, nfm;   // reference score, PBIAS - f m
+    float m;        // reference score
     float l;        // this lane group's part of the sum
 };
 
@@ -427,8 +427,7 @@ __device__ __forceinline__ void row_init(const Kv4AttnArgs& a, const Tile& t, in
     w.pos = (int)max(pos, -1L);
     w.lo = a.window > 0 ? (int)max(0L, pos - a.window + 1) : 0;
     w.f = f;
-    w.m = -__builtin_inff();
-    w.nfm = 0.0f;
+    w.m = -FLT_MAX;  // (finite: a masked score less it is -inf)
     w.l = t.bad ? __builtin_nanf("") : 0.0f;
 }
 
@@ -460,18 +459,25 @@ __device__ __forceinline__ float row_max(const Row& w, int key, int sink, f4v c[
     return rows_reduce(top, OpMax{});
 }
 
+// p = 2^(f (c - m) + PBIAS): the reference is taken from the score before it is
+// scaled.  (c f - m f with m f rounded on its own is a step of fp32 off, past
+// 2^27 more than p has room for: the largest p would be 0 or infinite.)
+__device__ __forceinline__ float prob(const Row& w, float c) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(c - w.m, w.f, PBIAS));
+}
 // The reference follows a unit's maximum, and acc and l the reference.  It
 // moves only when a maximum passes it by 2^PSLACK, so that most units leave
 // acc alone.
 __device__ __forceinline__ bool grows(const Row& w, float top) { return top > w.m && !(w.f * (top - w.m) <= PSLACK); }
 template <int MT>
 __device__ __forceinline__ float follow(Row& w, float top, f4v* acc) {  // what acc was multiplied by
-    const bool grow = grows(w, top);
-    // (a score past fp32's range gives p = inf and so NaN; with -inf here it would give 0)
-    const float nfm = grow ? fmaxf(PBIAS - w.f * top, -FLT_MAX) : w.nfm;
-    const float keep = !grow ? 1.0f : w.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(nfm - w.nfm);
-    if (grow) w.m = top;
-    w.nfm = nfm;
+    float keep = 1.0f;
+    if (grows(w, top)) {
+        // (a maximum past fp32's range: NaN, from here to the row's end)
+        const float m = fabsf(w.f * top) <= FLT_MAX ? top : __builtin_nanf("");
+        keep = __builtin_amdgcn_exp2f(w.f * (w.m - m));
+        w.m = m;
+    }
 #pragma unroll
     for (int m = 0; m < MT; m++) acc[m] *= keep;
     return keep;
@@ -483,7 +489,7 @@ __device__ __forceinline__ void probabilities(Row& w, const f4v c[4], h8v ph[2],
     for (int x = 0; x < 4; x++)
 #pragma unroll
         for (int y = 0; y < 4; y++) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y], w.f, w.nfm));
+            const float e = prob(w, c[x][y]);
             p[x >> 1][(x & 1) * 4 + y] = e;
             sum += e;
         }
@@ -599,7 +605,7 @@ __device__ __forceinline__ void join_blocks(const Kv4AttnArgs& a, const Shares& 
             float m[RU], sum[RU];
             f4v o[RU];
 #pragma unroll
-            for (int x = 0; x < RU; x++) m[x] = __builtin_inff(), sum[x] = 0.0f, o[x] = f4v{0, 0, 0, 0};
+            for (int x = 0; x < RU; x++) m[x] = -FLT_MAX, sum[x] = 0.0f, o[x] = f4v{0, 0, 0, 0};
             for (int b = sh.b0; b <= sh.b1; b += PB) {
                 f4v n[RU][PB], v[RU][PB];
 #pragma unroll
@@ -615,9 +621,9 @@ __device__ __forceinline__ void join_blocks(const Kv4AttnArgs& a, const Shares& 
 #pragma unroll
                     for (int y = 0; y < PB; y++) {
                         if (b + y > sh.b1 || n[x][y].x == 0.0f) continue;  // (no key seen)
-                        const float now = fminf(m[x], n[x][y].y);
-                        const float keep = sum[x] != 0.0f ? __builtin_amdgcn_exp2f(now - m[x]) : 0.0f;
-                        const float w = __builtin_amdgcn_exp2f(now - n[x][y].y);
+                        const float now = fmaxf(m[x], n[x][y].y), f = n[x][y].z;
+                        const float keep = sum[x] != 0.0f ? __builtin_amdgcn_exp2f(f * (m[x] - now)) : 0.0f;
+                        const float w = __builtin_amdgcn_exp2f(f * (n[x][y].y - now));
                         m[x] = now;
                         sum[x] = sum[x] * keep + w * n[x][y].x;
                         o[x] = o[x] * keep + v[x][y] * w;
@@ -637,40 +643,40 @@ __device__ __forceinline__ void join_blocks(const Kv4AttnArgs& a, const Shares& 
 // tiles m = w, w + W, ... in out.
 constexpr int tiles_of_wave(int hd, int w) { return hd / 16 > w ? hd / 16 / w : 1; }
 template <int HD, int W>
-__device__ __forceinline__ void join_waves(f4v* acc, float nfm, float& l, float* nfm_all, float* smem, f4v* out) {
+__device__ __forceinline__ void join_waves(f4v* acc, const Row& w, float& l, float* m_all, float* smem, f4v* out) {
     constexpr int MT = HD / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15;
-    l = rows_sum(l);
-    float* s_n = smem;                 // [W][16]
+    l = rows_sum(w.l);
+    float* s_m = smem;                 // [W][16]
     float* s_l = smem + 16 * W;        // [W][16]
-    f4v* s_o = (f4v*)(smem + 32 * W);  // [W][MT tiles][64 lanes], each to its own wave's maximum
+    f4v* s_o = (f4v*)(smem + 32 * W);  // [W][MT tiles][64 lanes], each to its own wave's reference
     __syncthreads();                   // the last piece's readers are done
     if (lane < 16) {
-        s_n[wave * 16 + i] = l != 0.0f ? nfm : __builtin_inff();  // no key seen: no weight (NaN counts as seen)
+        s_m[wave * 16 + i] = l != 0.0f ? w.m : -FLT_MAX;  // no key seen: no weight (NaN counts as seen)
         s_l[wave * 16 + i] = l;
     }
 #pragma unroll
     for (int m = 0; m < MT; m++) s_o[(wave * MT + m) * 64 + lane] = acc[m];
     __syncthreads();
-    float n = s_n[i];
+    float top = s_m[i];
 #pragma unroll
-    for (int w = 1; w < W; w++) n = fminf(n, s_n[w * 16 + i]);
+    for (int v = 1; v < W; v++) top = fmaxf(top, s_m[v * 16 + i]);
     float sum = 0.0f, f[W];
 #pragma unroll
-    for (int w = 0; w < W; w++) {
-        const float x = s_l[w * 16 + i];
-        f[w] = x != 0.0f ? __builtin_amdgcn_exp2f(n - s_n[w * 16 + i]) : 0.0f;
-        sum += x * f[w];
+    for (int v = 0; v < W; v++) {
+        const float x = s_l[v * 16 + i];
+        f[v] = x != 0.0f ? __builtin_amdgcn_exp2f(w.f * (s_m[v * 16 + i] - top)) : 0.0f;
+        sum += x * f[v];
     }
     l = sum;
-    *nfm_all = n;
+    *m_all = top;
 #pragma unroll
     for (int c = 0; c < tiles_of_wave(HD, W); c++) {
         const int m = c * W + wave;
         f4v o = {0, 0, 0, 0};
         if (m < MT)
 #pragma unroll
-            for (int w = 0; w < W; w++) o += s_o[(w * MT + m) * 64 + lane] * f[w];
+            for (int v = 0; v < W; v++) o += s_o[(v * MT + m) * 64 + lane] * f[v];
         out[c] = o;
     }
 }
@@ -831,9 +837,9 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
         if (more) begin();
 #pragma unroll
         for (int x = 0; x < NT; x++) {
-            float l = w[x].l, nfm;
+            float l, m;
             f4v o[tiles_of_wave(HD, W)];
-            join_waves<HD, W>(acc[x], w[x].nfm, l, &nfm, smem, o);
+            join_waves<HD, W>(acc[x], w[x], l, &m, smem, o);
             const int r = done.r0 + 16 * x + i;
             if (r >= done.r1 || wave >= MT) continue;
             if (!sh.split()) {
@@ -846,7 +852,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
                 const unsigned row = part_at<HD, R>(sh.slot(blockIdx.x), r - done.r0);
 #pragma unroll
                 for (int c = 0; c < tiles_of_wave(HD, W); c++) parts.put4(row + 16 * (c * W + wave) + 4 * g, o[c]);
-                if (wave == 0 && g == 0) parts.put4(row + HD, f4v{l, nfm, 0, 0});
+                if (wave == 0 && g == 0) parts.put4(row + HD, f4v{l, m, w[x].f, 0});
             }
         }
         if (sh.split()) shares.add(sh, done);
@@ -1065,12 +1071,12 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
                         for (int z = 0; z < 2; z++) {
                             float p[2];
 #pragma unroll
-                            for (int k = 0; k < 2; k++) p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][y][2 * z + k], w[x].f, w[x].nfm));
+                            for (int k = 0; k < 2; k++) p[k] = prob(w[x], c[x][y][2 * z + k]);
                             const Two t = split2(p[0], p[1]);
                             ph[x][y >> 1][2 * (y & 1) + z] = t.hi;
                             pl[x][y >> 1][2 * (y & 1) + z] = t.lo;
                         }
-                interleave(std::integral_constant<int, QM>(), std::integral_constant<int, 16 * NT * 5 / KS / QM>());
+                interleave(std::integral_constant<int, QM>(), std::integral_constant<int, 16 * NT * 4 / KS / QM>());
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int y = 0; y < 4; y++) cur[y] = nxt[y];
@@ -1138,7 +1144,7 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
                 float* row = a.part + part_at<HD, R>(sh.slot(blockIdx.x), r - t.r0);
 #pragma unroll
                 for (int m = 0; m < MT; m++) *(f4v*)(row + 16 * m + 4 * g) = acc[x][m];
-                if (g == 0) *(f4v*)(row + HD) = f4v{l, w[x].nfm, 0, 0};
+                if (g == 0) *(f4v*)(row + HD) = f4v{l, w[x].m, w[x].f, 0};
             }
         }
     } while (SPLIT && work.left > 0);
@@ -1159,7 +1165,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
     t.q0 = left.q0, t.head = left.head, t.r0 = left.r0, t.r1 = left.r1;
     const int l = threadIdx.x % LPR, r = t.r0 + (int)blockIdx.y * RPB + threadIdx.x / LPR;
     if (r < t.r1) {
-        float m = __builtin_inff(), sum = 0.0f;
+        float m = -FLT_MAX, sum = 0.0f;
         f4v o = {0, 0, 0, 0};
         for (int b = sh.b0; b <= sh.b1; b += PB) {
             f4v n[PB], v[PB];
@@ -1172,8 +1178,9 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
 #pragma unroll
             for (int y = 0; y < PB; y++) {
                 if (b + y > sh.b1 || n[y].x == 0.0f) continue;  // (no key seen)
-                const float now = fminf(m, n[y].y), keep = sum != 0.0f ? __builtin_amdgcn_exp2f(now - m) : 0.0f;
-                const float w = __builtin_amdgcn_exp2f(now - n[y].y);
+                const float now = fmaxf(m, n[y].y), f = n[y].z;
+                const float keep = sum != 0.0f ? __builtin_amdgcn_exp2f(f * (m - now)) : 0.0f;
+                const float w = __builtin_amdgcn_exp2f(f * (n[y].y - now));
                 m = now;
                 sum = sum * keep + w * n[y].x;
                 o = o * keep + v[y] * w;

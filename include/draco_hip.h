@@ -609,7 +609,8 @@ int draco_kv4_read(const DracoKv4* cache, const int* slot, int n, float* k, floa
  *
  * max_q, max_len: the largest row count and length of a sequence; other values
  * only cost speed.  A length past max_blocks pages, a page outside the pool
- * that a row sees, or a score past fp32's range gives NaN.
+ * that a row sees, or scores whose largest is past fp32's range give NaN
+ * (scaled to powers of two, 1.44 times themselves).
  *
  * work / work_bytes: draco_kv4_attn_workspace(cache, p) bytes, 16-byte
  * aligned, which depend on head_dim and the current device only: one

@@ -43,3 +43,72 @@ def test_probabilities_keep_22_bits(dev, hd, nh, nkv, m, code):  # noqa: F811
     want = (one * np.tanh(d) * np.where(p % 2, -1, 1)[:, None])[:, :, None]
     tol = 2.0 ** -19.9 + 6 * 2.0 ** -24 + np.abs(want) * (2.0 ** -24 if code == F32 else 2.0 ** -11) + (0 if code == F32 else 2.0 ** -25)
     assert (np.abs(out - want) <= tol).all(), np.abs(out - want).max()
+
+
+@pytest.mark.parametrize("hd,nh,nkv,m", KERNELS)
+@pytest.mark.parametrize("mag", [1e5, 1e8, 3e8, 1e9, 1e20, 1e35])
+def test_large_scores_pick_the_largest(dev, hd, nh, nkv, m, mag):  # noqa: F811
+    """q of any size: the key that wins by more than the scores' rounding is the output, to 2^-20; ties stay among the values.
+
+    A score is off by at most ds = big (2^-22 + (1.1 hd + 6) 2^-24) (two-term
+    q, the fp32 sums of its products, its scaling); where the second largest is
+    2 ds + 20 behind, all others weigh less than n e^-20 = 2^-19 of the first."""
+    rng = np.random.default_rng(hd + m)
+    n = m + 330
+    c = Cache(dev, [n], nkv, hd, 16)
+    k, v = (rng.standard_normal((n, nkv, hd)).astype(np.float32) for _ in range(2))
+    c.append(None, k, v, c.slots(0, 0, n))
+    kk, vv = R.quantize(k)[2], R.quantize(v)[2]
+    q = (rng.standard_normal((m, nh, hd)) * mag).astype(np.float32)
+    out = c.attn(q, [0, m], [n]).astype(np.float64)
+    clear = 0
+    for r in np.unique(np.concatenate([[0, m - 1], rng.integers(0, m, 12)])):
+        for h in (0, nh - 1):
+            g, p = h // (nh // nkv), n - m + r
+            x = q[r, h].astype(np.float64) * hd ** -0.5
+            s, big = kk[:p + 1, g] @ x, float((np.abs(kk[:p + 1, g]) @ np.abs(x)).max())
+            ds = big * (2.0 ** -22 + (1.1 * hd + 6) * 2.0 ** -24)
+            top, seen = int(s.argmax()), vv[:p + 1, g]
+            assert (out[r, h] >= seen.min(0) - 1e-5).all() and (out[r, h] <= seen.max(0) + 1e-5).all(), (r, h)
+            if s[top] - np.delete(s, top).max() > 2 * ds + 20:
+                clear += 1
+                assert np.abs(out[r, h] - seen[top]).max() <= (2.0 ** -19 + 2.0 ** -20) * np.abs(seen).max(), (r, h, s[top])
+    assert clear
+
+
+@pytest.mark.parametrize("hd,nh,nkv,m", KERNELS)
+@pytest.mark.parametrize("mag", [1, 1e8, 1e12, 1e30])
+def test_equal_scores_weigh_the_same(dev, hd, nh, nkv, m, mag):  # noqa: F811
+    """All keys alike: the output is the mean of the values seen, however large the scores are.
+
+    Equal keys have equal scores bit by bit, so p is 2^6 throughout; the sums
+    take a rounding of 2^-24 a key, twice, the division and two-term p 2^-21."""
+    rng = np.random.default_rng(hd + m)
+    n = m + 330
+    c = Cache(dev, [n], nkv, hd, 16)
+    k = np.tile(rng.standard_normal((1, nkv, hd)).astype(np.float32), (n, 1, 1))
+    v = rng.standard_normal((n, nkv, hd)).astype(np.float32)
+    c.append(None, k, v, c.slots(0, 0, n))
+    vv = R.quantize(v)[2]
+    q = (rng.standard_normal((m, nh, hd)) * mag).astype(np.float32)
+    out = c.attn(q, [0, m], [n]).astype(np.float64)
+    mean = (np.cumsum(vv, 0) / np.arange(1, n + 1)[:, None, None])[n - m:]
+    want = np.repeat(mean, nh // nkv, 1)
+    assert np.abs(out - want).max() <= (2 * (n + 16) * 2.0 ** -24 + 2.0 ** -21) * np.abs(vv).max()
+
+
+@pytest.mark.parametrize("hd,nh,nkv,m", [k for k in KERNELS if k[3] in (1, 7, 40, 1100)])
+def test_large_scores_of_f16_rows(dev, hd, nh, nkv, m):  # noqa: F811
+    """f16 rows reach scores of 1e10 too: one key is 1.25 times the others and wins."""
+    rng = np.random.default_rng(hd + m)
+    n = m + 330
+    c = Cache(dev, [n], nkv, hd, 16)
+    k, v = np.full((n, nkv, hd), 4.8e4, np.float32), rng.standard_normal((n, nkv, hd)).astype(np.float16).astype(np.float32)
+    win = 77
+    k[win] = 6e4
+    c.append(None, k, v, c.slots(0, 0, n), code=F16)
+    q = np.full((m, nh, hd), 6e4, np.float16)
+    q[:, 1::2] = 3e4
+    out = c.attn(q, [0, m], [n], code=F16).astype(np.float64)
+    want = np.repeat(R.quantize(v)[2][win], nh // nkv, 0)
+    assert (np.abs(out - want) <= np.abs(want) * 2.0 ** -11 + 2.0 ** -20).all()
