@@ -13,8 +13,10 @@
 // free as long as both operands share it).
 //
 // K and V values are exact in f16 (kv4.h).  p is split into two f16 terms, 22
-// bits, and so is q of fp32 rows (scaled by a power of two to [1, 2) of its
-// largest): their products run twice into one fp32 sum.  q of f16 rows is exact.
+// bits, and so is q of fp32 rows: their products run twice into one fp32 sum.  q
+// of f16 rows is exact.  A row of fp32 q is scaled by a power of two so that its
+// largest value lies just below f16's range: the second term ends at 2^-24, which
+// leaves 22 bits to every value down to 2^-17 of the largest.
 #include <float.h>
 #include <hip/hip_runtime.h>
 
@@ -375,9 +377,11 @@ __device__ __forceinline__ void cut_vpart(VPart& v, int key, int len) {
     }
 }
 
-// q rows of one 16-row tile as operands; f: 2^-e with max |q 2^e| in [1, 2),
-// times nothing else (the softmax scale is in q).  Lane (i, g): row i, dims in
-// the order of load_k's words.
+// q rows of one 16-row tile as operands, fp32 ones times 2^(QTOP - e) with 2^e
+// the power of two at or below the largest; f: the softmax scale less that, so
+// that f times a score of the operands is the exponent of 2.  Lane (i, g): row i,
+// dims in the order of load_k's words.
+constexpr int QTOP = 14;  // f16 ends below 2^16; the fp32 sums reach 2^(15 + 16 + 8)
 template <int HD, bool F16>
 __device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const Tile& t, int r, h8v* hi, h8v* lo, float& f) {
     constexpr int KS = HD / 32;
@@ -402,15 +406,15 @@ __device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const Tile& t, int 
         f = a.scale_log2;
     } else {
         top = rows_reduce(top, OpMax{});  // the row's other dims: the three other lane groups
-        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 126);
-        const float up = __uint_as_float((unsigned)(127 - e) << 23);
+        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, QTOP - 100), 126);
+        const float up = __uint_as_float((unsigned)(127 + QTOP - e) << 23);
 #pragma unroll
         for (int s = 0; s < KS; s++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[s][j] *= up;
             split8(x[s], hi[s], lo[s]);
         }
-        f = a.scale_log2 * __uint_as_float((unsigned)(127 + e) << 23);
+        f = a.scale_log2 * __uint_as_float((unsigned)(127 + e - QTOP) << 23);
     }
 }
 

@@ -604,8 +604,9 @@ int draco_kv4_read(const DracoKv4* cache, const int* slot, int n, float* k, floa
  * sequence), drafts and prompt chunks, mixed as they come.
  *
  * Whatever the rows' type and whichever kernel a batch takes: the pages' values
- * are used as they are, q of fp32 rows and the probabilities in 22 bits, sums
- * in fp32, and the result is rounded once, to the rows' type.
+ * are used as they are, q of fp32 rows (values down to 2^-17 of a row's largest)
+ * and the probabilities in 22 bits, sums in fp32, and the result is rounded
+ * once, to the rows' type.
  *
  * max_q, max_len: the largest row count and length of a sequence; other values
  * only cost speed.  A length past max_blocks pages, a page outside the pool

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import kv4_ref as R
-from test_gpu_kv4 import F16, F32, NP, Cache, dev  # noqa: F401 (dev is a fixture)
+from test_gpu_kv4 import F16, F32, NP, Cache, bound, dev  # noqa: F401 (dev is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,42 @@ def test_large_scores_of_f16_rows(dev, hd, nh, nkv, m):  # noqa: F811
     out = c.attn(q, [0, m], [n], code=F16).astype(np.float64)
     want = np.repeat(R.quantize(v)[2][win], nh // nkv, 0)
     assert (np.abs(out - want) <= np.abs(want) * 2.0 ** -11 + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("hd,nh,nkv,m", KERNELS)
+@pytest.mark.parametrize("far", [2.0 ** 6, 2.0 ** 10, 2.0 ** 14, 2.0 ** 17])
+def test_small_q_values_beside_large_ones(dev, hd, nh, nkv, m, far):  # noqa: F811
+    """As test_probabilities_keep_22_bits, with a q channel `far` times the largest other that meets K values of 0."""
+    rng = np.random.default_rng(hd + m)
+    n = m + 1
+    c = Cache(dev, [n], nkv, hd, 16)
+    k, v = np.zeros((n, nkv, hd), np.float32), np.ones((n, nkv, hd), np.float32)
+    k[:, :, 5] = rng.uniform(0.5, 2, (n, nkv)) * rng.choice([-1, 1], (n, nkv))
+    v[1::2] = -1
+    c.append(None, k, v, c.slots(0, 0, n))
+    kv, one = R.quantize(k)[2][:, :, 5], R.quantize(v)[2][0, 0, 0]
+    q = rng.uniform(0.5, 2, (m, nh, hd)).astype(np.float32)
+    q[:, :, 40] = rng.choice([-1, 1], (m, nh)) * far
+    out = c.attn(q, [0, m], [n], scale=0.125, window=2).astype(np.float64)
+    p = np.arange(1, n)
+    head = np.arange(nh) // (nh // nkv)
+    d = q[:, :, 5].astype(np.float64) * 0.125 * (kv[p][:, head] - kv[p - 1][:, head]) / 2
+    want = (one * np.tanh(d) * np.where(p % 2, -1, 1)[:, None])[:, :, None]
+    assert (np.abs(out - want) <= 2.0 ** -19.9 + 6 * 2.0 ** -24 + np.abs(want) * 2.0 ** -24).all(), np.abs(out - want).max()
+
+
+@pytest.mark.parametrize("hd,nh,nkv,m", [k for k in KERNELS if k[3] in (1, 7, 40, 1100)])
+def test_channels_of_opposite_size(dev, hd, nh, nkv, m):  # noqa: F811
+    """Channels where q is 2^14 times smaller and K as much larger: both halves make the score."""
+    rng = np.random.default_rng(hd + m)
+    n = m + 100
+    c = Cache(dev, [n], nkv, hd, 16)
+    size = np.where(np.arange(hd) < hd // 2, 2.0 ** 7, 2.0 ** -7)
+    k, v = ((rng.standard_normal((n, nkv, hd)) * x).astype(np.float32) for x in (size, 1))
+    c.append(None, k, v, c.slots(0, 0, n))
+    kk, vv = R.quantize(k)[2], R.quantize(v)[2]
+    q = (rng.standard_normal((m, nh, hd)) / size).astype(np.float32)
+    out = c.attn(q, [0, m], [n]).astype(np.float64)
+    for r in np.unique(np.concatenate([[0, m - 1], rng.integers(0, m, 12)])):
+        want, big = R.attention(q[r:r + 1], kk, vv, np.array([n - m + r]), hd ** -0.5, 0, 0)
+        assert np.abs(out[r] - want[0]).max() <= bound(F32, hd, n, big, np.abs(vv).max()), r
