@@ -11,7 +11,9 @@
 // last, behind every block's reads.
 //
 // Latency bound (a few KB): 8 sequences 4.2 us, 512 of up to 30000 tokens with
-// 39629 rows 6.9, a release of 300 4.7, of which about 2 are any launch's.
+// 39629 rows 6.9, a release of 300 6.8, of which about 2 are any launch's (and 2
+// are for entries that may be no pages: the counter waits for the table's
+// entries, and the list's stores pass the L2s).
 #include <hip/hip_runtime.h>
 #include <limits.h>
 
@@ -51,17 +53,20 @@ __device__ __forceinline__ Sum2 block_scan(Sum2 v, Sum2& total, long* red) {
 
 __device__ __forceinline__ int pages_of(long len, int sh) { return (int)((len + (1 << sh) - 1) >> sh); }
 
-// The last block to arrive (its counter left at 0 again); others return false.
-// Only reads lie before it, and a block's are done when it arrives.
-__device__ __forceinline__ bool last_block(int* ticket, int* flag) {
-    __syncthreads();
+// The blocks that arrived with a mark, in the last one to arrive (its counter
+// left at 0 again); -1 in the others.  A block's reads are done when it arrives,
+// and its writes where it has waited for them.
+__device__ __forceinline__ int last_block(int* ticket, bool mark, int* flag) {
+    mark = __syncthreads_or(mark);
     if (threadIdx.x == 0) {
-        const int n = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = n == (int)gridDim.x - 1;
-        if (*flag) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int add = mark ? 0x10001 : 1;  // (a grid has fewer than 2^15 blocks)
+        const int n = add + __hip_atomic_fetch_add(ticket, add, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = (n & 0xFFFF) == (int)gridDim.x;
+        *flag = last ? n >> 16 : -1;
+        if (last) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    return *flag != 0;
+    return *flag;
 }
 
 struct Seq {  // one sequence of a tile
@@ -156,7 +161,7 @@ __global__ __launch_bounds__(TILE) void k_kv_plan(KvPlanArgs a) {
     }
     if (a.n_seq == 0 && blockIdx.x == 0 && tid == 0) a.cu_q[0] = 0;
     // lengths and the list's count, behind every block's reads of them
-    if (gridDim.x > 1 && !last_block(a.ticket, &flag)) return;
+    if (gridDim.x > 1 && last_block(a.ticket, false, &flag) < 0) return;
     const long rows = row;
     long took = 0, refused = 0;
     row = page = 0;
@@ -200,7 +205,10 @@ __device__ __forceinline__ Rel release_seq(const KvReleaseArgs& a, int base, lon
 
 // The released pages' ordinals run over sequences and blocks as a plan's do;
 // page k of n goes to free_list[n_free + n - 1 - k], so that a release of what
-// a plan took restores the list.
+// a plan took restores the list.  An entry that is no page of the pool (one
+// behind a window, whose page the caller took back) leaves no gap: every block
+// places its entries as if all were pages, past the L2s, and the last one closes
+// the list up where a block met others.
 template <int TILE>
 __global__ __launch_bounds__(TILE) void k_kv_release(KvReleaseArgs a) {
     __shared__ long red[32];
@@ -212,6 +220,7 @@ __global__ __launch_bounds__(TILE) void k_kv_release(KvReleaseArgs a) {
     long all = 0, page = 0;
     Rel s = {};
     for (int base = 0; base < a.n_seq; base += TILE) s = release_seq<TILE>(a, base, all, red);
+    bool bad = false;
     for (int base = 0; base < a.n_seq; base += TILE) {
         if (a.n_seq > TILE) s = release_seq<TILE>(a, base, page, red);  // (else the tile's are still here)
         const int n = min(TILE, a.n_seq - base);
@@ -223,18 +232,80 @@ __global__ __launch_bounds__(TILE) void k_kv_release(KvReleaseArgs a) {
             for (int b = tid & 63; b < s_go[i]; b += 64) {
                 const long e = (long)(base + i) * a.max_blocks + s_want[i] + b;
                 const long at = n_free + all - 1 - (s_first[i] + b);
+                if (at >= a.n_pages) continue;  // (not all of them are pages)
                 const int p = a.block_table[e];
+                bad |= (unsigned)p >= (unsigned)a.n_pages;
                 a.block_table_out[e] = -1;
-                if (at < a.n_pages) a.free_list[at] = p;
+                __hip_atomic_store(a.free_list + at, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         if (base + TILE < a.n_seq) __syncthreads();
     }
-    if (gridDim.x > 1 && !last_block(a.ticket, &flag)) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last block may read what was stored
+    const int marks = gridDim.x > 1 ? last_block(a.ticket, bad, &flag) : __syncthreads_or(bad);
+    if (marks < 0) return;
+    const long end = min(n_free + all, (long)a.n_pages);
+    long count = end;
+    if (marks || n_free + all > end) {
+        // what was placed, closed up in its order
+        count = n_free;
+        for (long base = n_free; base < end; base += TILE) {
+            const long i = base + tid;
+            const int p = i < end ? __hip_atomic_load(a.free_list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : -1;
+            const bool ok = (unsigned)p < (unsigned)a.n_pages;
+            Sum2 sum;  // (its barriers lie between the tile's loads and stores)
+            const Sum2 in = block_scan<TILE>({ok, 0}, sum, red);
+            if (ok) a.free_list[count + in.a - 1] = p;
+            count += sum.a;
+        }
+        // the first ordinals, for which there was no room: counted, then placed behind the others
+        const long rest = n_free + all - end;
+        long left = 0;
+        for (int pass = 0; pass < 2; pass++) {
+            long seen = 0;
+            page = 0;
+            for (int base = 0; base < a.n_seq && page < rest; base += TILE) {
+                const long first = page;
+                s = release_seq<TILE>(a, base, page, red);
+                const int n = min(TILE, a.n_seq - base);
+                __syncthreads();
+                s_want[tid] = s.want;
+                s_first[tid] = s.first;
+                __syncthreads();
+                for (long k0 = first; k0 < min(page, rest); k0 += TILE) {
+                    const long k = k0 + tid;
+                    int p = -1;
+                    long e = 0;
+                    const bool mine = k < min(page, rest);
+                    if (mine) {
+                        int lo = 0, hi = n;  // the last sequence that starts at or before k
+                        while (hi - lo > 1) {
+                            const int mid = (lo + hi) >> 1;
+                            if (s_first[mid] <= k) lo = mid;
+                            else hi = mid;
+                        }
+                        e = (long)(base + lo) * a.max_blocks + s_want[lo] + (k - s_first[lo]);
+                        p = a.block_table[e];
+                    }
+                    const bool ok = (unsigned)p < (unsigned)a.n_pages;
+                    Sum2 sum;
+                    const Sum2 in = block_scan<TILE>({ok, 0}, sum, red);
+                    if (pass && mine) {
+                        const long at = count + left - (seen + in.a);
+                        if (ok && at < a.n_pages) a.free_list[at] = p;
+                        a.block_table_out[e] = -1;
+                    }
+                    seen += sum.a;
+                }
+            }
+            left = seen;
+        }
+        count = min(count + left, (long)a.n_pages);
+    }
     for (int base = 0; base < a.n_seq; base += TILE) {
         if (a.n_seq > TILE) s = release_seq<TILE>(a, base, page, red);
         if (base + tid < a.n_seq) a.kv_len_out[base + tid] = s.keep;
     }
-    if (tid == 0) *a.n_free_out = (int)min(n_free + all, (long)a.n_pages);
+    if (tid == 0) *a.n_free_out = (int)count;
 }
 
 }  // namespace

@@ -536,7 +536,9 @@ int draco_kv_plan(const DracoKvPlan* p, void* stream);
  * (0: it ended; less than it holds: drafted tokens taken back).  Pages behind
  * them go onto free_list and leave -1 in block_table_out (other entries are
  * not written; it may be block_table), in the reverse of a plan's order: a
- * release of what a plan just took restores the list.  kv_len_out = the tokens
+ * release of what a plan just took restores the list.  Entries outside the pool
+ * are no pages and do not go onto the list: a caller that takes back the pages
+ * behind a window itself leaves -1 in their place.  kv_len_out = the tokens
  * kept, n_free_out the list's new count; they may be kv_len / n_free.  `work`
  * as in draco_kv_plan. */
 typedef struct {
