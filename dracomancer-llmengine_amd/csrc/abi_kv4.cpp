@@ -219,6 +219,9 @@ int draco_kv4_append(const DracoKv4* cache, const DracoKv4Append* p, void* strea
     // q_out may be q itself (each value is written by the lane that read it
     // only where pairs are consecutive; halves read each other's)
     if (p->n_head && p->rot && p->pairing == 1 && p->q == p->q_out) return fail(-1, "%s: q_out is q with pairs in halves", who);
+    // .. and where a token's row of one is its row of the other
+    if (p->n_head && p->n_tok > 1 && p->q == p->q_out && p->q_stride != p->q_out_stride)
+        return fail(-1, "%s: q_out is q with strides %ld and %ld", who, p->q_stride, p->q_out_stride);
     a.q = p->q;
     a.k = p->k;
     a.v = p->v;

@@ -569,7 +569,8 @@ int draco_kv_release(const DracoKvRelease* p, void* stream);
  * four (time, height, width, ...), each with its own positions, pos_stride
  * ints apart.  Products and sums in 64 bits, one rounding to fp32 (f16 q:
  * another to f16).  A position outside the table makes its pairs NaN.  q_out
- * may be q with pairing 0 or rot 0 only, and overlaps no input otherwise.
+ * may be q with pairing 0 or rot 0 and equal strides only, and overlaps no input
+ * otherwise.
  *
  * A k or v row that is not finite is held as NaN: attention rows that see the
  * token become NaN, others do not.  Magnitudes past 65472 saturate. */

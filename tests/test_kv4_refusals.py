@@ -127,3 +127,11 @@ def test_one_workspace_size_serves_every_batch(hd):
     sizes = {L.draco_kv4_attn_workspace(ct.byref(c), ct.byref(attn(code=code, n_seq=s, n_tok=t, max_q=q, n_head=h)))
              for code in (7, 9) for s, t, q in ((0, 0, 1), (1, 1, 1), (3, 70, 50), (9, 4000, 4000)) for h in (2, 64)}
     assert len(sizes) == 1 and sizes.pop() >= 16384
+
+
+@pytest.mark.parametrize("pairing,rot", [(0, 64), (0, 0), (1, 0)])
+def test_append_in_place_needs_one_stride(pairing, rot):
+    """q rotated in place: rows of another stride would lie over other tokens' rows."""
+    kw = dict(q_out=P, pairing=pairing, rot=rot)
+    refused(L.draco_kv4_append(ct.byref(cache()), ct.byref(append(q_out_stride=264, **kw)), None), "q_out is q")
+    refused(L.draco_kv4_append(ct.byref(cache()), ct.byref(append(q_stride=264, **kw)), None), "q_out is q")
