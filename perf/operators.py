@@ -316,8 +316,11 @@ def _prepare_step(case, seed):
 
 
 def prepare(case, seed):
-    return {"plan": _prepare_pages, "release": _prepare_pages, "append": _prepare_append, "attn": _prepare_attn,
-            "step": _prepare_step}[case["kind"]](case, seed)
+    stream = _loop_stream() if own else None
+    s = {"plan": _prepare_pages, "release": _prepare_pages, "append": _prepare_append, "attn": _prepare_attn,
+         "step": _prepare_step}[case["kind"]](case, seed)
+    s.stream = stream
+    return s
 
 
 # ---- the library's calls --------------------------------------------------------
@@ -332,13 +335,20 @@ def _lib():
     return lib
 
 
-def _stream():
-    """The serving loop's stream."""
-    if not _streams:
-        s = torch.cuda.Stream()
-        s.wait_stream(torch.cuda.current_stream())
-        _streams.append(s)
-    return _streams[0].cuda_stream
+def _loop_stream():
+    """The one stream of a serving program, for its inputs, the calls and what reads their outputs: the current one.
+
+    The library takes the null stream for its own, which nothing of torch's is
+    ordered with: where the null stream is current, the loop's own becomes it.
+    """
+    s = torch.cuda.current_stream()
+    if s.cuda_stream == 0:
+        if not _streams:
+            _streams.append(torch.cuda.Stream())
+        _streams[0].wait_stream(s)
+        s = _streams[0]
+        torch.cuda.set_stream(s)
+    return s.cuda_stream
 
 
 def _own_plan(s):
@@ -389,13 +399,12 @@ def _own_attn(s, q, kv_len):
     cache = _own_cache(s)
     need = L.load().draco_kv4_attn_workspace(ct.byref(cache), ct.byref(a))
     s.attn_work = torch.zeros(max(16, need), dtype=torch.uint8, device=device)
-    torch.cuda.current_stream().synchronize()  # the workspace is cleared before another stream uses it
     a.work, a.work_bytes = s.attn_work.data_ptr(), need
     return L.load().draco_kv4_attn, ct.byref(cache), ct.byref(a)
 
 
-def _call(fn, *args):
-    rc = fn(*args, _stream())
+def _call(stream, fn, *args):
+    rc = fn(*args, stream)
     if rc:
         _lib().check(rc, fn.__name__)
 
@@ -419,7 +428,7 @@ def _run_own(s):
         s.call = s.call or [_own_plan(s), _own_append(s, s.n, s.rope, s.rows, [0] * (s.case["hd"] // 2), 1, True),
                             _own_attn(s, s.q_out, s.kv_out)]
     for c in s.call:
-        _call(*c)
+        _call(s.stream, *c)
 
 
 # ---- the plain forms ------------------------------------------------------------
