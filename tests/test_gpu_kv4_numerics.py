@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 # (head dim, q heads, KV heads, rows): rows of every kernel -- decode, two row
 # tiles at head dim 128, tiles of 64, whole tiles of 64, whole tiles of 128 / 256
 KERNELS = [(hd, 4, 1, m) for hd in (64, 128, 256) for m in (1, 7, 40)]
-KERNELS += [(64, 32, 4, 600), (128, 32, 4, 600), (256, 32, 4, 600), (64, 32, 4, 2100), (128, 32, 4, 1100), (256, 16, 2, 1100)]
+KERNELS += [(64, 32, 4, 600), (128, 32, 4, 600), (256, 32, 4, 600), (64, 32, 4, 2100), (64, 128, 4, 1100), (128, 32, 4, 1100), (256, 16, 2, 1100)]
 
 
 @pytest.mark.parametrize("hd,nh,nkv,m", KERNELS)
