@@ -453,8 +453,7 @@ __device__ __forceinline__ float row_max(const Row& w, int key, int sink, f4v c[
         for (int r = 0; r < 4; r++) {
             if constexpr (MASK) {
                 const int j = key + 4 * t + r;
-                // (& and |: with && the compiler branches, and where c lives in
-                // accumulation registers one such branch lost the value)
+                // (& and |: three comparisons and a select a score, no branch)
                 const bool see = (j <= w.pos) & ((j >= w.lo) | (j < sink));
                 c[t][r] = see ? c[t][r] : -__builtin_inff();
             }
