@@ -961,7 +961,7 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
         kp = page_of(a, t.table, k_key(unit_of(0)));
         vp = page_of(a, t.table, v_key(unit_of(0)));
         // this wave's rows; a wave without any repeats the tile's last and stores nothing
-        const int r0 = min(t.r0 + wave * 16 * NT, t.r1 - 1), r1 = min(t.r0 + (wave + 1) * 16 * NT, t.r1);
+        const int mine = t.r0 + wave * 16 * NT, r0 = min(mine, t.r1 - 1), r1 = min(mine + 16 * NT, t.r1);
         h8v qh[NT][KS], ql[NT][F16 ? 1 : KS];
         Row w[NT];
         f4v acc[NT][MT], c[NT][4], d[NT][4];
@@ -1136,7 +1136,7 @@ __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_att
 #pragma unroll
         for (int x = 0; x < NT; x++) {
             const float l = sum[x][0];
-            const int r = r0 + 16 * x + i;
+            const int r = mine + 16 * x + i;
             if (r >= r1) continue;
             if (!sh.split()) {
                 const float inv = l != 0.0f ? 1.0f / l : 0.0f;
