@@ -57,7 +57,7 @@ __device__ __forceinline__ int pages_of(long len, int sh) { return (int)((len + 
 // left at 0 again); -1 in the others.  A block's reads are done when it arrives,
 // and its writes where it has waited for them.
 __device__ __forceinline__ int last_block(int* ticket, bool mark, int* flag) {
-    mark = __syncthreads_or(mark);
+    __syncthreads();
     if (threadIdx.x == 0) {
         const int add = mark ? 0x10001 : 1;  // (a grid has fewer than 2^15 blocks)
         const int n = add + __hip_atomic_fetch_add(ticket, add, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -241,7 +241,8 @@ __global__ __launch_bounds__(TILE) void k_kv_release(KvReleaseArgs a) {
         if (base + TILE < a.n_seq) __syncthreads();
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last block may read what was stored
-    const int marks = gridDim.x > 1 ? last_block(a.ticket, bad, &flag) : __syncthreads_or(bad);
+    int marks = __syncthreads_or(bad);
+    if (gridDim.x > 1) marks = last_block(a.ticket, marks != 0, &flag);
     if (marks < 0) return;
     const long end = min(n_free + all, (long)a.n_pages);
     long count = end;
