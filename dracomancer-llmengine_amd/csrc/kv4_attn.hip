@@ -692,11 +692,11 @@ __device__ __forceinline__ void join_waves(f4v* acc, const Row& w, float& l, flo
 // one 64th a lane and pass through LDS, which takes 8 wide loads and 32
 // registers less than loading them to every lane.
 // HBM bound where the batch is long: 64 sequences of up to 16384 keys, 32 / 4
-// heads of 128, fp32 rows, 395 MB in 95 us (4.15 TB/s; a copy reaches 4.80).
+// heads of 128, fp32 rows, 395 MB in 96 us (4.12 TB/s; a copy reaches 4.80).
 // Short ones are a chain of latencies: 1000 keys of 32 / 8 heads of 64 9 us.
 // One unit in flight a wave: two made hardly more of the bandwidth and much
 // more code, which every block fetches first (24 sequences of 16 / 2 heads of
-// 256, window 6001: 41 us against 47).
+// 256, window 6001: 43 us, 47 with two).
 template <int HD>
 struct Raw {
     KRow<HD, HD / 32> k[4];
@@ -872,12 +872,14 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(Kv4AttnArgs a) {
 // exponentials of unit n among the products of unit n + 1's scores, and stages
 // later units' operands among unit n's output products.  K operands are staged
 // two units ahead and V operands one; one barrier a turn.
-// 2048 rows of 32 / 4 heads of 128 over 8192 keys: f16 378 us, 361 GFLOP of
-// products issued (p's second term makes them three for two), 954 TFLOP/s, where
-// a library product of 8192^3 reaches 1123; fp32 433 us, 481 GFLOP, 1111.  Two
-// row tiles a wave do not fit the registers there (f16 441 us, 31 spilled).
-// With p as one f16 an f16 call took 273 us, and its rows were off by up to
-// 2^-11 of the values before their own rounding.
+// 2048 rows of 32 / 4 heads of 128 over 8192 keys: f16 391 us, 361 GFLOP of
+// products issued (p's second term makes them three for two), 923 TFLOP/s, where
+// a library product of 8192^3 reaches 1123; fp32 445 us, 481 GFLOP, 1081.  The
+// matrix units are busy 40 % of the time, vector instructions issue in 55 %, and
+// the two overlap little: bound by their sum.  Two row tiles a wave do not fit
+// the registers there (f16 441 us, 31 spilled).  With p as one f16 the f16 call
+// took 273 us, and its rows were off by up to 2^-11 of the values before their
+// own rounding.
 template <int HD, bool F16, int W, int NT, bool SPLIT>
 __global__ __launch_bounds__(64 * W, HD == 256 && W == 4 ? 1 : 2) void k_kv4_attn_prompt(Kv4AttnArgs a) {
     constexpr int KS = HD / 32, MT = HD / 16, R = 16 * NT * W;
@@ -1217,11 +1219,12 @@ void attn_run(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
 // every batch).  Measured on 256 CUs, us:
 // - up to 16 rows a sequence and KV head the decode kernel, whose waves share
 //   nothing but the rows; more rows would read the pages once per 16 of them.
-// - up to 32 at head dim 128 the same with two row tiles (356 registers, so one
-//   block a CU): 24 sequences of 5 drafts over 20011 keys, window 6001, 32 / 8
-//   heads, 76 against 116 in tiles of 64 in fp32 and 75 against 102 in f16.
-//   At 64 (12 drafts of 32 / 8 heads over 8000 keys 73 against 55) and at 256,
-//   where they spill (5 drafts 98 against 71), the tiles of 64 are faster.
+// - up to 32 at head dim 128 the same with two row tiles (352 registers in f16,
+//   387 in fp32, so one block a CU): 24 sequences of 5 drafts over 20011 keys,
+//   window 6001, 32 / 8 heads, 76 against 116 in tiles of 64 in fp32 and 75
+//   against 102 in f16.  At 64 (12 drafts of 32 / 8 heads over 8000 keys 73
+//   against 55) and at 256, where they spill (5 drafts 98 against 71), the tiles
+//   of 64 are faster.
 // - tiles of 64 rows, and of 128 (256 at head dim 64; at 256 in fp32 the
 //   registers leave no larger one) where there is one for every CU: 2048 rows of
 //   32 / 4 heads of 128 over 8192 keys 409 against 435 in f16, 461 against 487 in
