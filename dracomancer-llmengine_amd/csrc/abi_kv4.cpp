@@ -112,8 +112,9 @@ int batch_ok(int n_seq, int max_blocks, int n_pages, int page_size, const char* 
     return 0;
 }
 
+int too_large(const char* who) { return fail(-1, "%s: the batch needs more blocks than a launch has", who); }
 int launched(int rc, const char* who) {
-    if (rc) return fail(-1, "%s: the batch needs more blocks than a launch has", who);
+    if (rc) return too_large(who);
     DRACO_HIP(hipGetLastError());
     return 0;
 }
@@ -239,6 +240,7 @@ int draco_kv4_append(const DracoKv4* cache, const DracoKv4Append* p, void* strea
     a.pos_stride = p->n_axes > 1 ? p->pos_stride : 0;
     a.table = p->table;
     a.table_rows = p->table_rows;
+    if (kv4_append_grid(a).blocks > KV4_MAX_GRID) return too_large(who);
     OnDevice dev;
     hipStream_t st;
     if (int rc = dev.enter(stream, &st)) return rc;
@@ -254,6 +256,7 @@ int draco_kv4_read(const DracoKv4* cache, const int* slot, int n, float* k, floa
     if (n == 0) return 0;
     if (!slot || !k || !v) return fail(-1, "%s: null pointer", who);
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(-1, "%s: k or v is not 16-byte aligned", who);
+    if (kv4_read_grid(c, n) > KV4_MAX_GRID) return too_large(who);
     OnDevice dev;
     hipStream_t st;
     if (int rc = dev.enter(stream, &st)) return rc;

@@ -47,7 +47,15 @@ struct Kv4AppendArgs {
     uint32_t axis[8];    // of pair i: bits 2 (i % 16) .. of word i / 16
     int kv_passes;       // (filled by kv4_append)
 };
-int kv4_append(const Kv4AppendArgs& a, bool f16, bool halves, hipStream_t st);
+// Blocks of 256 threads of a launch, at most: it has fewer than 2^32 threads.
+constexpr long KV4_MAX_GRID = 0xFFFFFF;
+struct Kv4AppendGrid {
+    long kv, blocks;  // blocks that write K and V, all
+    int kv_passes;
+};
+Kv4AppendGrid kv4_append_grid(const Kv4AppendArgs& a);
+long kv4_read_grid(const Kv4View& c, int n);
+int kv4_append(Kv4AppendArgs a, bool f16, bool halves, hipStream_t st);
 int kv4_read(const Kv4View& c, const int* slot, int n, float* k, float* v, hipStream_t st);
 
 struct Kv4AttnArgs {

@@ -278,16 +278,9 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4View c, const int* slots, i
 }
 
 template <int HD>
-int append_hd(Kv4AppendArgs a, bool f16, bool halves, hipStream_t st) {
-    constexpr int RPB = 256 / (HD / 8) * QU;  // q heads a block
-    constexpr int KPB = 256 / (HD / 4);       // K and V rows a pass
-    a.kv_passes = (long)a.n_tok / KV_TOKENS * a.c.n_kv >= 1024 ? KV_TOKENS / KPB : 1;
-    const int per = KPB * a.kv_passes;
-    const long kv = ((long)a.n_tok + per - 1) / per * a.c.n_kv;
-    const long grid = kv + (long)a.n_tok * ((a.n_head + RPB - 1) / RPB);
-    if (grid > 0x7FFFFFFFL) return -1;
-    const dim3 gr((unsigned)grid), bl(256);
-    const unsigned n = (unsigned)kv;
+int append_hd(const Kv4AppendArgs& a, const Kv4AppendGrid& g, bool f16, bool halves, hipStream_t st) {
+    const dim3 gr((unsigned)g.blocks), bl(256);
+    const unsigned n = (unsigned)g.kv;
     if (f16 && halves) hipLaunchKernelGGL((k_kv4_append<HD, true, true>), gr, bl, 0, st, a, n);
     else if (f16) hipLaunchKernelGGL((k_kv4_append<HD, true, false>), gr, bl, 0, st, a, n);
     else if (halves) hipLaunchKernelGGL((k_kv4_append<HD, false, true>), gr, bl, 0, st, a, n);
@@ -297,19 +290,37 @@ int append_hd(Kv4AppendArgs a, bool f16, bool halves, hipStream_t st) {
 
 }  // namespace
 
-int kv4_append(const Kv4AppendArgs& a, bool f16, bool halves, hipStream_t st) {
+Kv4AppendGrid kv4_append_grid(const Kv4AppendArgs& a) {
+    const int rpb = 256 / (a.c.hd / 8) * QU;  // q heads a block
+    const int kpb = 256 / (a.c.hd / 4);       // K and V rows a pass
+    Kv4AppendGrid g;
+    g.kv_passes = (long)a.n_tok / KV_TOKENS * a.c.n_kv >= 1024 ? KV_TOKENS / kpb : 1;
+    const int per = kpb * g.kv_passes;
+    g.kv = ((long)a.n_tok + per - 1) / per * a.c.n_kv;
+    g.blocks = g.kv + (long)a.n_tok * ((a.n_head + rpb - 1) / rpb);
+    return g;
+}
+
+int kv4_append(Kv4AppendArgs a, bool f16, bool halves, hipStream_t st) {
+    const Kv4AppendGrid g = kv4_append_grid(a);
+    if (g.blocks > KV4_MAX_GRID) return -1;
+    a.kv_passes = g.kv_passes;
     switch (a.c.hd) {
-    case 64: return append_hd<64>(a, f16, halves, st);
-    case 128: return append_hd<128>(a, f16, halves, st);
-    case 256: return append_hd<256>(a, f16, halves, st);
+    case 64: return append_hd<64>(a, g, f16, halves, st);
+    case 128: return append_hd<128>(a, g, f16, halves, st);
+    case 256: return append_hd<256>(a, g, f16, halves, st);
     }
     return -1;
 }
 
-int kv4_read(const Kv4View& c, const int* slot, int n, float* k, float* v, hipStream_t st) {
+long kv4_read_grid(const Kv4View& c, int n) {
     const int rpb = 256 / (c.hd / 4);
-    const long grid = ((long)n * c.n_kv + rpb - 1) / rpb;
-    if (grid > 0x7FFFFFFFL) return -1;
+    return ((long)n * c.n_kv + rpb - 1) / rpb;
+}
+
+int kv4_read(const Kv4View& c, const int* slot, int n, float* k, float* v, hipStream_t st) {
+    const long grid = kv4_read_grid(c, n);
+    if (grid > KV4_MAX_GRID) return -1;
     const dim3 gr((unsigned)grid), bl(256);
     switch (c.hd) {
     case 64: hipLaunchKernelGGL(k_kv4_read<64>, gr, bl, 0, st, c, slot, n, k, v); return 0;

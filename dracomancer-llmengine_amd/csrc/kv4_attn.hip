@@ -1272,7 +1272,7 @@ size_t kv4_attn_workspace(int hd, int cus) {
 }
 
 int kv4_attn(Kv4AttnArgs a, bool f16, const Kv4AttnPlan& p, void* work, hipStream_t st) {
-    if (p.grid > 0x7FFFFFFFL) return -1;
+    if (p.grid > KV4_MAX_GRID / (p.rows > 64 ? 2 : 1)) return -1;  // (512 threads from 128 rows on)
     a.whole = p.whole;
     a.part_bytes = (unsigned)p.part_bytes;
     a.chunk = p.chunk;

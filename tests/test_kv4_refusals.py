@@ -135,3 +135,11 @@ def test_append_in_place_needs_one_stride(pairing, rot):
     kw = dict(q_out=P, pairing=pairing, rot=rot)
     refused(L.draco_kv4_append(ct.byref(cache()), ct.byref(append(q_out_stride=264, **kw)), None), "q_out is q")
     refused(L.draco_kv4_append(ct.byref(cache()), ct.byref(append(q_stride=264, **kw)), None), "q_out is q")
+
+
+def test_more_threads_than_a_launch_has():
+    """2^24 blocks of 256 threads are one too many."""
+    c = cache()
+    refused(L.draco_kv4_append(ct.byref(c), ct.byref(append(n_tok=1 << 26, pos_stride=1 << 26)), None), "more blocks")
+    refused(L.draco_kv4_append(ct.byref(c), ct.byref(append(n_tok=1 << 28, n_head=0, rot=0)), None), "more blocks")
+    refused(L.draco_kv4_read(ct.byref(c), P, 1 << 28, P, P, None), "more blocks")
