@@ -11,7 +11,7 @@
 // last, behind every block's reads.
 //
 // Latency bound (a few KB): 8 sequences 4.2 us, 512 of up to 30000 tokens with
-// 39629 rows 6.9, a release of 300 6.8, of which about 2 are any launch's (and 2
+// 39629 rows 6.9, a release of 300 6.7, of which about 2 are any launch's (and 2
 // are for entries that may be no pages: the counter waits for the table's
 // entries, and the list's stores pass the L2s).
 #include <hip/hip_runtime.h>
